@@ -163,6 +163,56 @@ int32_t nc_matmul_i8_token_stacked(void **p, const int64_t *s);
  * GEMV 7, or an MFMA tile 16..24) */
 int32_t nc_matmul_i8_token_swiglu(void **p, const int64_t *s);
 
+/* -- microscaled (MX) 4-bit weights ---------------------------------------------
+ * Blocks of 32 values of a row share one scale byte, a power of two's exponent
+ * plus 127 (255: NaN), times elements of 4 bits (e2m1) or 8 (e4m3), as the Open
+ * Compute Project's Microscaling Formats specification has them. No counterpart
+ * in the reference, whose narrowest weights are int8 (quantize.py:55-70). A row of K values
+ * is padded with zeros to steps = ceil(K / 128) times 128: codes u8[rows, steps * 16 * bits]
+ * (two 4-bit elements a byte, the lower index in the low bits), scales
+ * u8[rows, steps * 4]. Codes lie on 16-byte boundaries, scales on 4-byte ones
+ * (others are refused); float32 operands on any boundary of a float. */
+
+/* Rows to MX: a block's scale puts its largest value into the elements' top
+ * binade (floor(log2(max|x|)) - 2 or - 8, at least -127), each value times the inverse
+ * goes to the nearest element, ties to even, past the largest to that. A block that
+ * holds a NaN or an infinity has scale NaN and zero elements. Every step is
+ * exact but the rounding to elements: the codes are the definition's, bit for bit.
+ * p: [codes, scales, x f32[M,K]];  s: [M, K, bits (4 or 8)] */
+int32_t nc_quantize_mx(void **p, const int64_t *s);
+
+/* The values MX rows stand for (exact unless past float32's range).
+ * p: [x f32[M,K], codes, scales];  s: [M, K, bits (4 or 8)] */
+int32_t nc_dequantize_mx(void **p, const int64_t *s);
+
+/* A residual's addition, rms_norm and a quantizer in one pass: t = x + delta
+ * (x without delta), n = (t * r) * gamma with r = 1 / sqrt(sum(t * t) / K + eps)
+ * taken in 64 bits and rounded to float32 once, then n quantized: format 0
+ * int8 with a scale a token (nc_quantize_token_i8's arithmetic, for
+ * nc_matmul_i8_token), 4 or 8 MX elements of that many bits (nc_quantize_mx's,
+ * for nc_matmul_mx). The codes do not depend on the order of the sum. sum, the
+ * new residual stream, may be x or delta; q and normed overlap no input.
+ * (nc_rms_norm_quant sums in float32 in an order of its own: r may differ in its last bit.)
+ * p: [sum f32[M,K] or NULL, normed f32[M,K] or NULL, q i8[M,K] or codes, qs f32[M] or scales,
+ *     x f32[M,K], delta f32[M,K] or NULL, gamma f32[K]];
+ * s: [M, K (at most 32768), eps as float32 bits, format] */
+int32_t nc_add_rms_norm_quant(void **p, const int64_t *s);
+
+/* y = x @ w.T of MX activations (of 4 or 8 bits) and MX 4-bit weights, added in
+ * float32 on the scaled matrix cores, then + bias, then residual + y. A row that
+ * holds a NaN scale gives NaN outputs; y may be the residual, and overlaps no
+ * other operand.
+ * p: [y f32[M,N], xq codes, xs scales, q codes of N rows, scales of N rows,
+ *     bias f32[N] or NULL, residual f32[M,N] or NULL];
+ * s: [M, N, K, bits of xq (4 or 8)] (M * N < 2^40) */
+int32_t nc_matmul_mx(void **p, const int64_t *s);
+
+/* SwiGLU's gate and up projections sharing one pass over the activations, then
+ * h = silu(gate) * up, the products as nc_matmul_mx's.
+ * p: [h f32[M,N], xq codes, xs scales, qg codes, sg scales, qu codes, su scales];
+ * s: [M, N, K, bits of xq (4 or 8)] (M * N < 2^40) */
+int32_t nc_matmul_mx_swiglu(void **p, const int64_t *s);
+
 /* -- the reference's own int8 modes, bit for bit ------------------------------ */
 
 /* matmul_i8: y = x @ (q * scales).T with f32 activations times int8 weights,

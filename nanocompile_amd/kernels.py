@@ -14,14 +14,14 @@ import numpy as np
 from nanocompile_amd import hip
 from nanocompile_amd.hip import DeviceArray
 
-F32, I8, I32 = np.dtype(np.float32), np.dtype(np.int8), np.dtype(np.int32)
+F32, I8, I32, U8 = (np.dtype(t) for t in (np.float32, np.int8, np.int32, np.uint8))
 
 
 class ShapeError(ValueError):
     """Operands that do not fit the primitive (the reference's ir.ShapeError)."""
 
 
-SHORT = {F32: "f32", I8: "i8", I32: "i32", np.dtype(np.int64): "i64"}
+SHORT = {F32: "f32", I8: "i8", I32: "i32", U8: "u8", np.dtype(np.int64): "i64"}
 
 
 def _device(x, dtype=None) -> DeviceArray:
@@ -167,6 +167,121 @@ def matmul_i8_token_stacked(xq, xs, q, scales, out: DeviceArray | None = None, s
         out = DeviceArray((b, m, n), F32)
     hip.call("nc_matmul_i8_token_stacked", [out, xq, xs, q, scales], [b, m, n, k, schedule])
     return out
+
+
+# -- microscaled (MX) 4-bit weights -----------------------------------------------------
+
+
+def mx_widths(k: int, bits: int) -> tuple[int, int]:
+    """Bytes of codes and of scales a row of ``k`` values has: rows are padded to multiples of 128 values."""
+    steps = -(-k // 128)
+    return steps * 16 * bits, steps * 4
+
+
+def _operand(op: str, name: str, x, dtype, shape) -> DeviceArray:
+    """``x`` on the device, checked before any copy: its dtype, and each size that ``shape`` gives (None: any)."""
+    have = x if isinstance(x, DeviceArray) else np.asarray(x)
+    if have.dtype != dtype or len(have.shape) != len(shape) or any(
+            want is not None and want != got for want, got in zip(shape, have.shape)):
+        want = ", ".join("*" if d is None else str(d) for d in shape)
+        raise ShapeError(f"{op}: {name} must be {SHORT[np.dtype(dtype)]}[{want}], got "
+                         f"{SHORT.get(have.dtype, str(have.dtype))}{list(have.shape)}")
+    return have if isinstance(have, DeviceArray) else DeviceArray.from_host(have)
+
+
+def _mx_bits(op: str, codes, scales) -> int:
+    """The bits of an element of ``codes: u8[M, steps * 16 * bits]``, ``scales: u8[M, steps * 4]``."""
+    shapes = [tuple(x.shape) if hasattr(x, "shape") else np.shape(x) for x in (codes, scales)]
+    if all(len(s) == 2 for s in shapes) and shapes[0][0] == shapes[1][0]:
+        for bits in (4, 8):
+            if shapes[1][1] and shapes[1][1] % 4 == 0 and shapes[0][1] == 4 * bits * shapes[1][1]:
+                return bits
+    raise ShapeError(f"{op}: expected codes u8[M, steps * 64 or * 128] and scales u8[M, steps * 4], "
+                     f"got {list(shapes[0])}, {list(shapes[1])}")
+
+
+def quantize_mx(x, bits: int = 4) -> tuple[DeviceArray, DeviceArray]:
+    """``x: f32[M, K]`` to MX elements of 4 (e2m1) or 8 (e4m3) bits: ``(codes, scales)``, rows padded to 128 values."""
+    if bits not in (4, 8):
+        raise ValueError(f"MX elements have 4 or 8 bits, got {bits!r}")
+    x = _operand("quantize_mx", "x", x, F32, (None, None))
+    m, k = x.shape
+    width, blocks = mx_widths(k, bits)
+    codes, scales = DeviceArray((m, width), U8), DeviceArray((m, blocks), U8)
+    if m and k:
+        hip.call("nc_quantize_mx", [codes, scales, x], [m, k, bits])
+    return codes, scales
+
+
+def dequantize_mx(codes, scales, k: int) -> DeviceArray:
+    """The first ``k`` values a row that MX ``codes`` and ``scales`` stand for: f32[M, k]."""
+    bits = _mx_bits("dequantize_mx", codes, scales)
+    width, blocks = mx_widths(k, bits)
+    codes = _operand("dequantize_mx", "codes", codes, U8, (None, width))
+    scales = _operand("dequantize_mx", "scales", scales, U8, (None, blocks))
+    m = codes.shape[0]
+    x = DeviceArray((m, k), F32)
+    if m:
+        hip.call("nc_dequantize_mx", [x, codes, scales], [m, k, bits])
+    return x
+
+
+def add_rms_norm_quant(x, delta, gamma, eps: float, mx_bits: int = 0, normed: bool = False):
+    """``t = x + delta`` (``delta`` None: x), ``rms_norm(t) * gamma`` and its quantized form, one kernel:
+    ``(t, normed | None, q, qs)``. ``mx_bits`` 0 is int8 with a scale a token (for :func:`matmul_i8_token`),
+    4 or 8 MX codes and scales (for :func:`matmul_mx`)."""
+    if mx_bits not in (0, 4, 8):
+        raise ValueError(f"mx_bits must be 0 (int8), 4 or 8, got {mx_bits!r}")
+    op = "add_rms_norm_quant"
+    x = _operand(op, "x", x, F32, (None, None))
+    m, k = x.shape
+    if delta is not None:
+        delta = _operand(op, "delta", delta, F32, (m, k))
+    gamma = _operand(op, "gamma", gamma, F32, (k,))
+    t = x if delta is None else DeviceArray((m, k), F32)
+    out = DeviceArray((m, k), F32) if normed else None
+    if mx_bits:
+        width, blocks = mx_widths(k, mx_bits)
+        q, qs = DeviceArray((m, width), U8), DeviceArray((m, blocks), U8)
+    else:
+        q, qs = DeviceArray((m, k), I8), DeviceArray((m,), F32)
+    if m:
+        hip.call("nc_add_rms_norm_quant", [None if delta is None else t, out, q, qs, x, delta, gamma],
+                 [m, k, float_bits(eps), mx_bits])
+    return t, out, q, qs
+
+
+def matmul_mx(xq, xs, q, scales, bias=None, residual=None) -> DeviceArray:
+    """``x @ w.T (+ bias) (+ residual)`` of MX activations (``quantize_mx`` in 4 or 8 bits) and MX 4-bit weights."""
+    op = "matmul_mx"
+    bits = _mx_bits(op, xq, xs)
+    m, blocks = xs.shape
+    xq, xs = _operand(op, "xq", xq, U8, (m, 4 * bits * blocks)), _operand(op, "xs", xs, U8, (m, blocks))
+    scales = _operand(op, "scales", scales, U8, (None, blocks))
+    n = scales.shape[0]
+    q = _operand(op, "q", q, U8, (n, 16 * blocks))
+    if bias is not None:
+        bias = _operand(op, "bias", bias, F32, (n,))
+    if residual is not None:
+        residual = _operand(op, "residual", residual, F32, (m, n))
+    y = DeviceArray((m, n), F32)
+    hip.call("nc_matmul_mx", [y, xq, xs, q, scales, bias, residual], [m, n, 32 * blocks, bits])
+    return y
+
+
+def matmul_mx_swiglu(xq, xs, qg, sg, qu, su) -> DeviceArray:
+    """``silu(x @ g.T) * (x @ u.T)`` of MX activations and two MX 4-bit weights, one kernel."""
+    op = "matmul_mx_swiglu"
+    bits = _mx_bits(op, xq, xs)
+    m, blocks = xs.shape
+    xq, xs = _operand(op, "xq", xq, U8, (m, 4 * bits * blocks)), _operand(op, "xs", xs, U8, (m, blocks))
+    sg = _operand(op, "sg", sg, U8, (None, blocks))
+    n = sg.shape[0]
+    su = _operand(op, "su", su, U8, (n, blocks))
+    qg, qu = _operand(op, "qg", qg, U8, (n, 16 * blocks)), _operand(op, "qu", qu, U8, (n, 16 * blocks))
+    h = DeviceArray((m, n), F32)
+    hip.call("nc_matmul_mx_swiglu", [h, xq, xs, qg, sg, qu, su], [m, n, 32 * blocks, bits])
+    return h
 
 
 # -- the reference's two int8 modes (matmul_i8, matmul_i8_vnni) ----------------------
