@@ -27,6 +27,7 @@ typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 using nc::f32x4;
+using nc::f32x4_any;
 
 struct MxArgs {
     float *y;                        // may be the residual
@@ -91,6 +92,12 @@ __device__ __forceinline__ Block<8> block_of(i32x4 lo, i32x4 hi, int scale) {
     return b;
 }
 
+template <int BITS>
+__device__ __forceinline__ Block<BITS> x_block(const i32x4 (&codes)[BITS / 4], int scale) {
+    if constexpr (BITS == 4) return block_of<4>(codes[0], scale);
+    else return block_of(codes[0], codes[1], scale);
+}
+
 // c + the products of a step. The compiler does not know that a scaled matrix instruction needs every lane, and may
 // move one whose result is used under a lane's condition under that condition: `pin` keeps results outside.
 __device__ __forceinline__ f32x4 mx_step(const Block<4> &w, const Block<4> &x, f32x4 c) {
@@ -106,88 +113,210 @@ __device__ __forceinline__ f32x4 mx_step(const Block<8> &w, const Block<8> &x, f
 
 __device__ __forceinline__ void pin(f32x4 &v) { asm volatile("" : "+v"(v)); }
 
-// A lane's block of x at `p` in memory.
-template <int BITS>
-__device__ __forceinline__ Block<BITS> load_x(const uint8_t *p, int scale) {
-    const i32x4 *q = reinterpret_cast<const i32x4 *>(p);
-    if constexpr (BITS == 4) return block_of<4>(q[0], scale);
-    else return block_of(q[0], q[1], scale);
-}
-
-// Outputs n .. n + 3 of row m from their sums (and for the pair those of the second weight).
+// Outputs n .. n + 3 of row m from their sums (and for the pair those of the second weight). Four at once where
+// the row has them: global memory takes wide loads and stores on any boundary of a float.
 template <int NB>
-__device__ __forceinline__ void finish(const MxArgs &a, int64_t m, int64_t n, f32x4 g, f32x4 u) {
-    if (m >= a.M) return;
+__device__ __forceinline__ void finish(const MxArgs &a, int64_t m, int64_t n, f32x4 v, f32x4 u) {
+    if (m >= a.M || n >= a.N) return;
     const size_t at = (size_t)m * a.N + n;
+    if constexpr (NB == 2) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        if (n + r >= a.N) return;
-        float v = g[r];
-        if constexpr (NB == 2) {
-            v = nc::silu_mul(v, u[r]);
-        } else {
-            if (a.bias) v = __fadd_rn(v, a.bias[n + r]);
-            if (a.residual) v = __fadd_rn(a.residual[at + r], v);
+        for (int r = 0; r < 4; ++r) v[r] = nc::silu_mul(v[r], u[r]);
+    }
+    if (n + 4 <= a.N) {
+        if constexpr (NB == 1) {
+            const f32x4 bias = a.bias ? *reinterpret_cast<const f32x4_any *>(a.bias + n) : f32x4{};
+            const f32x4 residual = a.residual ? *reinterpret_cast<const f32x4_any *>(a.residual + at) : f32x4{};
+            if (a.bias) v += bias;
+            if (a.residual) v = residual + v;
         }
-        a.y[at + r] = v;
+        *reinterpret_cast<f32x4_any *>(a.y + at) = v;
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 3; ++r) {
+        if (n + r >= a.N) return;
+        float w = v[r];
+        if constexpr (NB == 1) {
+            if (a.bias) w = __fadd_rn(w, a.bias[n + r]);
+            if (a.residual) w = __fadd_rn(a.residual[at + r], w);
+        }
+        a.y[at + r] = w;
     }
 }
 
-constexpr int kWaves = 4;
+// Workgroup id to tile: the 8 XCDs (workgroup i runs on XCD i % 8) take a contiguous range of tiles each, so that
+// the tiles of a band of weight rows, which follow one another, share an L2.
+__device__ __forceinline__ int64_t tile_of(int64_t id, int64_t total) {
+    return id < (total & ~(int64_t)7) ? (id & 7) * (total >> 3) + (id >> 3) : id;
+}
 
-// A workgroup takes 16 rows of x by 16 weight rows (of each weight), its waves a share of k each; the sums are
-// added in the order of the waves. Rows past M or N are the last one, their results not stored.
-template <int BITS, int NB>
-__global__ __launch_bounds__(kWaves * 64) void mx_few_rows(MxArgs a) {
-    const int64_t mtiles = (a.M + 15) / 16, tiles = mtiles * ((a.N + 15) / 16);
-    const int64_t tile = nc::workgroup_id();
-    if (tile >= tiles) return;
-    const int64_t m0 = tile % mtiles * 16, n0 = tile / mtiles * 16;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
-    const int64_t m = min(m0 + row, a.M - 1), n = min(n0 + row, a.N - 1);
-    const uint8_t *xq = a.xq + (size_t)m * a.steps * 16 * BITS + g * 4 * BITS, *xs = a.xs + (size_t)m * a.steps * 4 + g;
+// 16 bytes a lane from memory straight to LDS, at `to` + 16 * lane (`to` the same for every lane).
+__device__ __forceinline__ void copy_to_lds(const uint8_t *from, uint8_t *to) {
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) const void *)from,
+                                     (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
+// Staging of 16 rows by a step in LDS, ROW bytes a row. A lane's block lies 16 rows from its neighbours' in memory: read
+// as it is multiplied, 16 lanes that go through the cache together would touch 16 lines. So lanes copy whole row
+// segments, ROW / 16 of them a row, and the 16-byte chunks of row r are permuted by (r / 2) mod that number, which
+// keeps the reads of 16 rows at one chunk free of bank conflicts.
+template <int ROW>
+struct Stage {
+    static constexpr int kChunks = ROW / 16, kCopies = ROW / 64;     // copies of 1 KB
+    // The row, and byte in it, that a lane copies (the copy's rows before it not counted).
+    static __device__ __forceinline__ int row(int lane) { return lane / kChunks; }
+    static __device__ __forceinline__ int column(int lane, int copy) {
+        return (lane % kChunks ^ swizzle(copy * (16 / kCopies) + row(lane))) * 16;
+    }
+    static __device__ __forceinline__ int swizzle(int row) { return row / 2 % kChunks; }
+    // Where chunk c of row r lies.
+    static __device__ __forceinline__ int at(int r, int c) { return r * ROW + (c ^ swizzle(r)) * 16; }
+};
+
+// Few outputs: a workgroup takes 16 MF rows of x by 16 NF weight rows (of each weight), its waves a share of k each,
+// every wave through LDS of its own, U steps' copies in flight at once; the sums are added in the order of the waves.
+// Rows past M or N are the last one, their results not stored.
+template <int BITS, int NB, int MF, int NF, int WAVES, int U>
+__global__ __launch_bounds__(WAVES * 64) void mx_split(MxArgs a) {
+    using W = Stage<64>;
+    using X = Stage<16 * BITS>;
+    constexpr int kStep = 1024 * (NB * NF + MF * X::kCopies), kParts = WAVES * NB * MF * NF * 1024;
+    __shared__ __align__(1024) uint8_t lds[WAVES * U * kStep > kParts ? WAVES * U * kStep : kParts];
+
+    const int64_t mtiles = (a.M + 16 * MF - 1) / (16 * MF), tiles = mtiles * ((a.N + 16 * NF - 1) / (16 * NF));
+    if (nc::workgroup_id() >= tiles) return;
+    const int64_t tile = tile_of(nc::workgroup_id(), tiles);
+    const int64_t m0 = tile % mtiles * (16 * MF), n0 = tile / mtiles * (16 * NF);
+    const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), steps = a.steps;
+    // The tile's first rows and a step's place in them are the same for every lane (scalar registers); a lane's
+    // row and chunk are an offset of 32 bits.
+    auto x_row = [&](int r) { return (uint32_t)min((int64_t)r, a.M - 1 - m0) * (uint32_t)steps; };
+    auto w_row = [&](int r) { return (uint32_t)min((int64_t)r, a.N - 1 - n0) * (uint32_t)steps; };
+    const uint8_t *xq = a.xq + (size_t)m0 * steps * (16 * BITS), *xs = a.xs + (size_t)m0 * steps * 4;
     const uint8_t *q[NB], *ws[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        q[b] = a.q[b] + (size_t)n * a.steps * 64 + g * 16;
-        ws[b] = a.ws[b] + (size_t)n * a.steps * 4 + g;
+        q[b] = a.q[b] + (size_t)n0 * steps * 64;
+        ws[b] = a.ws[b] + (size_t)n0 * steps * 4;
     }
-    f32x4 acc[NB] = {};
-    const int share = (a.steps + kWaves - 1) / kWaves, begin = wave * share, end = min(a.steps, begin + share);
-    for (int s = begin; s < end; ++s) {
-        const Block<BITS> x = load_x<BITS>(xq + (size_t)s * 16 * BITS, xs[s * 4]);
+    uint32_t xat[MF][X::kCopies], xsat[MF], wat[NF], wsat[NF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+#pragma unroll
+        for (int h = 0; h < X::kCopies; ++h)
+            xat[i][h] = x_row(16 * i + h * (16 / X::kCopies) + X::row(lane)) * (16 * BITS) + X::column(lane, h);
+        xsat[i] = x_row(16 * i + row) * 4;
+    }
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+        wat[j] = w_row(16 * j + W::row(lane)) * 64 + W::column(lane, 0);
+        wsat[j] = w_row(16 * j + row) * 4;
+    }
+    f32x4 acc[NB][MF][NF] = {};
+    uint8_t *mine = lds + wave * U * kStep;
+    auto batch = [&](int s, auto count) {
+        constexpr int C = decltype(count)::value;
+        typedef uint32_t words __attribute__((ext_vector_type(C == 1 ? 2 : C), aligned(4)));
+        words xe[MF], we[NB][NF];
+        auto load_words = [&](const uint8_t *p) {
+            if constexpr (C == 1) return words{*reinterpret_cast<const uint32_t *>(p), 0u};
+            else return *reinterpret_cast<const words *>(p);
+        };
 #pragma unroll
         for (int b = 0; b < NB; ++b)
-            acc[b] = mx_step(
-                block_of<BITS>(*reinterpret_cast<const i32x4 *>(q[b] + (size_t)s * 64), ws[b][s * 4]), x, acc[b]);
-    }
-    __shared__ f32x4 part[kWaves][NB][64];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        pin(acc[b]);
-        part[wave][b][lane] = acc[b];
+            for (int j = 0; j < NF; ++j) we[b][j] = load_words(ws[b] + (size_t)s * 4 + wsat[j]);
+#pragma unroll
+        for (int i = 0; i < MF; ++i) xe[i] = load_words(xs + (size_t)s * 4 + xsat[i]);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int j = 0; j < NF; ++j)
+                    copy_to_lds(q[b] + (size_t)(s + c) * 64 + wat[j], mine + c * kStep + (b * NF + j) * 1024);
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int h = 0; h < X::kCopies; ++h)
+                    copy_to_lds(xq + (size_t)(s + c) * (16 * BITS) + xat[i][h],
+                                mine + c * kStep + (NB * NF + i * X::kCopies + h) * 1024);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const uint8_t *at = mine + c * kStep;
+            Block<BITS> x[MF];
+#pragma unroll
+            for (int i = 0; i < MF; ++i) {
+                i32x4 codes[BITS / 4];
+#pragma unroll
+                for (int h = 0; h < BITS / 4; ++h)
+                    codes[h] = *reinterpret_cast<const i32x4 *>(at + (NB * NF + i * X::kCopies) * 1024 +
+                                                                X::at(row, g * (BITS / 4) + h));
+                x[i] = x_block<BITS>(codes, xe[i][c] >> (8 * g) & 255);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int j = 0; j < NF; ++j) {
+                    const Block<BITS> w = block_of<BITS>(
+                        *reinterpret_cast<const i32x4 *>(at + (b * NF + j) * 1024 + W::at(row, g)),
+                        we[b][j][c] >> (8 * g) & 255);
+#pragma unroll
+                    for (int i = 0; i < MF; ++i) acc[b][i][j] = mx_step(w, x[i], acc[b][i][j]);
+                }
+        }
+    };
+    const int share = (steps + WAVES - 1) / WAVES, end = min(steps, (wave + 1) * share);
+    int s = wave * share;
+    for (; s + U <= end; s += U) batch(s, std::integral_constant<int, U>{});
+    if constexpr (U > 2) {
+        if (s + 2 <= end) batch(s, std::integral_constant<int, 2>{}), s += 2;
     }
-    __syncthreads();
-    if (wave > 0) return;
-    f32x4 sum[2] = {};
+    if constexpr (U > 1) {
+        if (s < end) batch(s, std::integral_constant<int, 1>{});
+    }
+    __syncthreads();                                   // every wave is done with its stage
+    f32x4 *part = reinterpret_cast<f32x4 *>(lds);      // [WAVES][NB][MF * NF][64]
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) sum[b] += part[w][b][lane];
-    finish<NB>(a, m0 + row, n0 + 4 * g, sum[0], sum[1]);
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int j = 0; j < NF; ++j) {
+                pin(acc[b][i][j]);
+                part[((wave * NB + b) * MF * NF + i * NF + j) * 64 + lane] = acc[b][i][j];
+            }
+    __syncthreads();
+    for (int f = wave; f < MF * NF; f += WAVES) {
+        f32x4 sum[2] = {};
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) sum[b] += part[((w * NB + b) * MF * NF + f) * 64 + lane];
+        finish<NB>(a, m0 + f / NF * 16 + row, n0 + f % NF * 16 + 4 * g, sum[0], sum[1]);
+    }
 }
 
-template <int NB>
-int32_t launch(const MxArgs &a, int64_t bits) {
-    const int64_t tiles = (a.M + 15) / 16 * ((a.N + 15) / 16);
-    auto *kernel = bits == 4 ? &mx_few_rows<4, NB> : &mx_few_rows<8, NB>;
-    hipLaunchKernelGGL(kernel, nc::grid_of(tiles), dim3(kWaves * 64), 0, nc::stream(), a);
-    return nc::launched("mx_few_rows");
+template <int BITS, int NB, int MF, int NF, int WAVES, int U>
+int32_t launch_split(const MxArgs &a) {
+    const int64_t tiles = (a.M + 16 * MF - 1) / (16 * MF) * ((a.N + 16 * NF - 1) / (16 * NF));
+    hipLaunchKernelGGL((mx_split<BITS, NB, MF, NF, WAVES, U>), nc::grid_of(tiles), dim3(WAVES * 64), 0, nc::stream(), a);
+    return nc::launched("mx_split");
 }
 
-// Shapes whose outputs are fewer than 2^40 (a terabyte of float32 is 2^38).
+template <int BITS, int NB>
+int32_t launch(const MxArgs &a) {
+    if (a.M > 16) return launch_split<BITS, NB, 2, 2, 4, 2>(a);
+    return a.steps >= 16 ? launch_split<BITS, NB, 1, 1, 8, 2>(a) : launch_split<BITS, NB, 1, 1, 4, 2>(a);
+}
+
+// Shapes whose outputs are fewer than 2^40 (a terabyte of float32 is 2^38) and whose rows a tile addresses in 32 bits.
 bool mx_matmul_shape(const int64_t *s) {
-    return s[0] >= 0 && s[1] > 0 && s[2] > 0 && s[0] < (1 << 26) && s[1] < (1 << 26) && s[2] < (1 << 26) &&
+    return s[0] >= 0 && s[1] > 0 && s[2] > 0 && s[0] < (1 << 26) && s[1] < (1 << 26) && s[2] <= (1 << 24) &&
            s[0] * s[1] < (int64_t)1 << 40;
 }
 
@@ -204,7 +333,7 @@ NC_EXPORT int32_t nc_matmul_mx(void **p, const int64_t *s) {
     const MxArgs a{(float *)p[0], (const uint8_t *)p[1], (const uint8_t *)p[2],
                    {(const uint8_t *)p[3], nullptr}, {(const uint8_t *)p[4], nullptr},
                    (const float *)p[5], (const float *)p[6], s[0], s[1], (int)(nc::mx_padded(s[2]) / nc::kMxPad)};
-    return launch<1>(a, s[3]);
+    return s[3] == 4 ? launch<4, 1>(a) : launch<8, 1>(a);
 }
 
 // p: [h f32[M,N], xq, xs, qg, sg, qu, su];  s: [M, N, K, bits of xq]
@@ -219,5 +348,5 @@ NC_EXPORT int32_t nc_matmul_mx_swiglu(void **p, const int64_t *s) {
     const MxArgs a{(float *)p[0], (const uint8_t *)p[1], (const uint8_t *)p[2],
                    {(const uint8_t *)p[3], (const uint8_t *)p[5]}, {(const uint8_t *)p[4], (const uint8_t *)p[6]},
                    nullptr, nullptr, s[0], s[1], (int)(nc::mx_padded(s[2]) / nc::kMxPad)};
-    return launch<2>(a, s[3]);
+    return s[3] == 4 ? launch<4, 2>(a) : launch<8, 2>(a);
 }

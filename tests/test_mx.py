@@ -109,7 +109,7 @@ def test_refusals(call, name):
         bits = at == len(sizes) - 1
         if name == "nc_add_rms_norm_quant" and at == 2:
             continue                                       # eps: any float
-        for bad in (-1, 1 << 26) if at == 0 else (3, 5, 16) if bits else (0, -1, 1 << 26):
+        for bad in (-1, 1 << 26) if at == 0 else (0, -1, (1 << 24) + 1) if at == 2 and "matmul" in name else (3, 5, 16) if bits else (0, -1, 1 << 26):
             refused("bits" if bits and name != "nc_add_rms_norm_quant" else "format" if bits else "bad shape", at,
                     size=bad)
     for at in CODES[name]:
