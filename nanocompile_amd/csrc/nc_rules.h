@@ -176,4 +176,14 @@ constexpr int prefill_rows(int64_t M, int64_t heads, int64_t kv_heads, int64_t k
     return group <= 4 && (M + 3) / 4 * ((keys + 63) / 64) * heads <= 1200 ? 4 : 0;
 }
 
+// The kernel of a microscaled product of M rows by N weight rows over `steps` of 128 values of k (nc_mx_matmul.hip).
+enum class MxTile { kRow, kLongRow, kSplit, kSmall, kLarge };
+
+constexpr MxTile mx_tile(int64_t M, int64_t N, int64_t steps, int bits, int weights) {
+    if (M <= 16) return steps >= 16 ? MxTile::kLongRow : MxTile::kRow;
+    const int64_t tiles = (M + 63) / 64 * ((N + 63) / 64) * weights;
+    if (steps < 4 || tiles < 256) return MxTile::kSplit;
+    return tiles < 4096 ? MxTile::kSmall : MxTile::kLarge;
+}
+
 }  // namespace nc

@@ -245,14 +245,19 @@ SHAPES = [(1, 1, 1), (1, 17, 32), (2, 16, 129), (3, 203, 100), (15, 64, 896), (1
           (129, 128, 4864), (257, 384, 896)]
 
 
+# many outputs: ragged in rows, columns and steps of 128 (4 to 9 of them)
+WIDE = [(1100, 1000, 513), (1030, 1024, 896), (1025, 1090, 768), (1089, 1030, 512), (1030, 1027, 1100), (300, 5003, 640),
+        (4100, 4130, 520), (4097, 4099, 896), (4128, 4100, 1024)]
+
+
 @pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("m,n,k", SHAPES + WIDE)
 def test_matmul(gpu, m, n, k, bits):
     check_matmul(m, n, k, bits)
 
 
 @pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("m,n,k", SHAPES + WIDE)
 def test_swiglu(gpu, m, n, k, bits):
     check_swiglu(m, n, k, bits)
 
@@ -278,7 +283,7 @@ def test_every_position_of_k_counts_once(gpu, m, bits):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("m,n,k", [(1, 100, 896), (40, 70, 300), (200, 300, 256)])
+@pytest.mark.parametrize("m,n,k", [(1, 100, 896), (40, 70, 300), (200, 300, 256), (1030, 1100, 640)])
 def test_bad_blocks_stay_in_their_rows(gpu, m, n, k, bits):
     """A NaN block of x spoils its row of y, one of w its column, and no other output changes a bit."""
     from nanocompile_amd import kernels
@@ -297,7 +302,7 @@ def test_bad_blocks_stay_in_their_rows(gpu, m, n, k, bits):
         assert np.array_equal(float_bits_of(got[i][~bad]), float_bits_of(clean[i][~bad]))
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 50, 200), (20, 51, 896), (130, 260, 640)])
+@pytest.mark.parametrize("m,n,k", [(1, 50, 200), (20, 51, 896), (130, 260, 640), (1030, 1101, 640)])
 def test_residual_in_place_and_guards(gpu, m, n, k):
     """y over the residual, on an address of a float, and nothing written outside it."""
     from nanocompile_amd import hip, kernels
