@@ -204,13 +204,13 @@ int32_t nc_add_rms_norm_quant(void **p, const int64_t *s);
  * other operand.
  * p: [y f32[M,N], xq codes, xs scales, q codes of N rows, scales of N rows,
  *     bias f32[N] or NULL, residual f32[M,N] or NULL];
- * s: [M, N, K, bits of xq (4 or 8)] (M * N < 2^40, K at most 2^24) */
+ * s: [M, N, K, bits of xq (4 or 8)] (M * N < 2^39, K at most 2^24) */
 int32_t nc_matmul_mx(void **p, const int64_t *s);
 
 /* SwiGLU's gate and up projections sharing one pass over the activations, then
  * h = silu(gate) * up, the products as nc_matmul_mx's.
  * p: [h f32[M,N], xq codes, xs scales, qg codes, sg scales, qu codes, su scales];
- * s: [M, N, K, bits of xq (4 or 8)] (M * N < 2^40, K at most 2^24) */
+ * s: [M, N, K, bits of xq (4 or 8)] (M * N < 2^39, K at most 2^24) */
 int32_t nc_matmul_mx_swiglu(void **p, const int64_t *s);
 
 /* -- the reference's own int8 modes, bit for bit ------------------------------ */

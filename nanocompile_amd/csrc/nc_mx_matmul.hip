@@ -55,42 +55,38 @@ struct Block<8> {
     bf16x8 part[4];
 };
 
+// Eight values to bfloat16: 4-bit codes in a word, 8-bit ones in two.
+__device__ __forceinline__ bf16x8 to_bf16(int codes, float power) {
+    const bf16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power, 0),
+                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power, 1),
+                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power, 2),
+                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power, 3)};
+    return __builtin_bit_cast(bf16x8, v);
+}
+__device__ __forceinline__ bf16x8 to_bf16(int low, int high, float power) {
+    const bf16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(low, power, false),
+                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(low, power, true),
+                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, power, false),
+                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, power, true)};
+    return __builtin_bit_cast(bf16x8, v);
+}
+
 // From 4-bit codes.
 template <int BITS>
 __device__ __forceinline__ Block<BITS> block_of(i32x4 codes, int scale) {
     if constexpr (BITS == 4) {
         return {codes, scale};
     } else {
-        Block<8> b;
         const float p = power(scale);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            bf16x2 v[4];
-            v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[t], p, 0);
-            v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[t], p, 1);
-            v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[t], p, 2);
-            v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[t], p, 3);
-            b.part[t] = __builtin_bit_cast(bf16x8, v);
-        }
-        return b;
+        return {{to_bf16(codes[0], p), to_bf16(codes[1], p), to_bf16(codes[2], p), to_bf16(codes[3], p)}};
     }
 }
 
 // From 8-bit codes, the block's first 16 and its last.
-__device__ __forceinline__ Block<8> block_of(i32x4 lo, i32x4 hi, int scale) {
-    Block<8> b;
+__device__ __forceinline__ Block<8> block_of(i32x4 low, i32x4 high, int scale) {
     const float p = power(scale);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int w0 = t < 2 ? lo[2 * t] : hi[2 * t - 4], w1 = t < 2 ? lo[2 * t + 1] : hi[2 * t - 3];
-        bf16x2 v[4];
-        v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, p, false);
-        v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, p, true);
-        v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, p, false);
-        v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, p, true);
-        b.part[t] = __builtin_bit_cast(bf16x8, v);
-    }
-    return b;
+    return {{to_bf16(low[0], low[1], p), to_bf16(low[2], low[3], p), to_bf16(high[0], high[1], p),
+             to_bf16(high[2], high[3], p)}};
 }
 
 template <int BITS>
@@ -170,10 +166,16 @@ __device__ __forceinline__ void finish(const MxArgs &a, int64_t m, int apart, in
     }
 }
 
-// Workgroup id to tile: the 8 XCDs (workgroup i runs on XCD i % 8) take a contiguous range of tiles each, so that
-// the tiles of a band of weight rows, which follow one another, share an L2.
-__device__ __forceinline__ int64_t tile_of(int64_t id, int64_t total) {
-    return id < (total & ~(int64_t)7) ? (id & 7) * (total >> 3) + (id >> 3) : id;
+// Workgroup id to tile: the 8 XCDs (workgroup i runs on XCD i % 8) take a contiguous range of tiles each, in an order
+// whose neighbours share operands in that XCD's L2: 8 tiles down the rows of x, then the next weight rows.
+struct Tile {
+    int64_t m, n;
+};
+__device__ __forceinline__ Tile tile_of(uint32_t id, uint32_t mtiles, uint32_t ntiles) {
+    const uint32_t total = mtiles * ntiles;
+    if (id < (total & ~7u)) id = (id & 7) * (total >> 3) + (id >> 3);
+    const uint32_t band = id / (8 * ntiles), down = min(8u, mtiles - band * 8), in = id - band * 8 * ntiles;
+    return {band * 8 + in % down, in / down};
 }
 
 // 16 bytes a lane from memory straight to LDS, at `to` + 16 * lane (`to` the same for every lane).
@@ -196,9 +198,10 @@ struct Stage {
     static __device__ __forceinline__ int row(int lane, int copy) {
         return copy / kCopies * 16 + copy % kCopies * (16 / kCopies) + lane / kChunks;
     }
+    static __device__ __forceinline__ int slot(int lane, int copy) { return lane % kChunks ^ swizzle(row(lane, copy)); }
     static __device__ __forceinline__ int column(int lane, int copy) {
-        const int slot = lane % kChunks ^ swizzle(row(lane, copy));
-        return (ROW == 64 ? slot : slot % 4 * 2 + slot / 4) * 16;
+        const int s = slot(lane, copy);
+        return (ROW == 64 ? s : s % 4 * 2 + s / 4) * 16;
     }
     // Where half h (0 in 4 bits) of block b of row r lies, counted from the first of these rows.
     static __device__ __forceinline__ int at(int r, int b, int h) { return r * ROW + ((b + 4 * h) ^ swizzle(r)) * 16; }
@@ -214,16 +217,17 @@ __global__ __launch_bounds__(WAVES * 64) void mx_split(MxArgs a) {
     constexpr int kStep = 1024 * (NB * NF + MF * X::kCopies), kParts = WAVES * NB * MF * NF * 1024;
     __shared__ __align__(1024) uint8_t lds[WAVES * U * kStep > kParts ? WAVES * U * kStep : kParts];
 
-    const int64_t mtiles = (a.M + 16 * MF - 1) / (16 * MF), tiles = mtiles * ((a.N + 16 * NF - 1) / (16 * NF));
-    if (nc::workgroup_id() >= tiles) return;
-    const int64_t tile = tile_of(nc::workgroup_id(), tiles);
-    const int64_t m0 = tile % mtiles * (16 * MF), n0 = tile / mtiles * (16 * NF);
+    const uint32_t mtiles = ((uint32_t)a.M + 16 * MF - 1) / (16 * MF), ntiles = ((uint32_t)a.N + 16 * NF - 1) / (16 * NF);
+    if (nc::workgroup_id() >= mtiles * ntiles) return;
+    const Tile tile = tile_of((uint32_t)nc::workgroup_id(), mtiles, ntiles);
+    const int64_t m0 = tile.m * (16 * MF), n0 = tile.n * (16 * NF);
     const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), steps = a.steps;
     // The tile's first rows and a step's place in them are the same for every lane (scalar registers); a lane's
     // row and chunk are an offset of 32 bits.
-    auto x_row = [&](int r) { return (uint32_t)min((int64_t)r, a.M - 1 - m0) * (uint32_t)steps; };
-    auto w_row = [&](int r) { return (uint32_t)min((int64_t)r, a.N - 1 - n0) * (uint32_t)steps; };
+    const int x_last = (int)min(a.M - 1 - m0, (int64_t)16 * MF - 1), w_last = (int)min(a.N - 1 - n0, (int64_t)16 * NF - 1);
+    auto x_row = [&](int r) { return (uint32_t)(min(r, x_last) * steps); };
+    auto w_row = [&](int r) { return (uint32_t)(min(r, w_last) * steps); };
     const uint8_t *xq = a.xq + (size_t)m0 * steps * (16 * BITS), *xs = a.xs + (size_t)m0 * steps * 4;
     const uint8_t *q[NB], *ws[NB];
 #pragma unroll
@@ -343,57 +347,46 @@ int32_t launch_split(const MxArgs &a) {
     return nc::launched("mx_split");
 }
 
-// c + the products of 64 values of k of 32 weight rows by 32 rows of x, lane l the row l % 32 of each and a block; the
-// outputs are acc[n = 8 (r / 4) + 4 (l / 32) + r % 4][m = l % 32].
-template <int OP>
-__device__ __forceinline__ f32x16 mx_half_step(const Block<4> &w, const Block<4> &x, f32x16 c) {
-    const i32x8 w8 = __builtin_shufflevector(w.codes, w.codes, 0, 1, 2, 3, -1, -1, -1, -1);
-    const i32x8 x8 = __builtin_shufflevector(x.codes, x.codes, 0, 1, 2, 3, -1, -1, -1, -1);
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w8, x8, c, 4, 4, OP, w.scale, OP, x.scale);
-}
-template <int OP>
-__device__ __forceinline__ f32x16 mx_half_step(const Block<8> &w, const Block<8> &x, f32x16 c) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.part[t], x.part[t], c, 0, 0, 0);
-    return c;
-}
-
 // copy_to_lds for copies that stay in flight past LDS reads: before any read of LDS the compiler waits for every copy it
 // knows of, as each might write what is read. Which copies a read needs is counted in mx_tile, so these are hidden
 // from it. They write no register; `to` goes through m0, which takes a wait state.
 __device__ __forceinline__ void copy_to_lds_counted(const uint8_t *from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "m0", "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from),
+                 "s"(__builtin_amdgcn_readfirstlane(to)) : "m0", "memory");
 }
 
-// Many outputs: a workgroup of WM x WN waves takes 32 MF WM rows of x by 32 NF WN weight rows (of each weight), staged in
-// a ring of four steps in LDS, each wave 32 MF x 32 NF of them from registers, half a step at a time: while one half
-// is multiplied the next is read, and the copies of two steps more are in flight. A wave waits until only the copies
-// issued after the next step's are left, and at the barrier for the other waves'. The scales come four steps at a
-// time, 16 bytes a row. The outputs go through LDS, a wave's 32 rows at a time, so that whole lines are written (a lane's own
-// outputs are 16 bytes of a row: 4096 x 8192 x 8192 took 255 us so, 140 of them without the stores). Needs four steps.
-template <int BITS, int NB, int WM, int WN, int MF, int NF>
+// Many outputs: a workgroup of WM x WN waves takes 32 MF WM rows of x by 32 NF WN weight rows (of each weight), each wave
+// 32 MF x 32 NF of them. Operands are staged in LDS two steps at a time, in two buffers: 4-bit rows are copied 128
+// bytes at a time, as whole lines of the cache come twice as fast as halves (measured: 33 against 16 TB/s). A wave
+// reads half a step's operands into registers while it multiplies the half before. One barrier a pair of steps, before
+// its last half: by then the next pair has landed and this one is read, so the copies of the pair after next start,
+// with two steps to land. Where the steps are odd the last is the second of a pair whose first is not multiplied again.
+// The scales come four steps at a time, 16 bytes a row, with the pairs 0, 2, 4 ... The outputs go through LDS, a wave's
+// 32 rows at a time, so that whole lines are written (a lane's own outputs are 16 bytes of a row: 4096 x 8192 x 8192
+// took 255 us so, 140 of them without the stores). Needs four steps.
+template <int BITS, int NB, int WM, int WN, int MF, int NF, int BUFFERS>
 __global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
-    using W = Stage<64, 4>;
-    using X = Stage<16 * BITS, BITS == 4 ? 4 : 2>;
+    using S = Stage<128, 2>;
     constexpr int WAVES = WM * WN, BM = 32 * MF * WM, BN = 32 * NF * WN, XH = BITS / 4;
-    constexpr int XC = BM / 16 * X::kCopies, WC = BN / 16, SC = (BM + NB * BN) / 64;   // copies a stage, a group
-    constexpr int BUFFER = (XC + NB * WC) * 1024;
-    constexpr int kCopies = (XC + NB * WC) / WAVES, kScaleCopies = (SC + WAVES - 1) / WAVES;      // a wave's
+    constexpr int XC = BM / 8, WC = BN / 8, SC = (BM + NB * BN) / 64;       // copies of 128-byte rows; of a group of scales
+    constexpr int BUFFER = (XH * XC + NB * WC) * 1024;
+    constexpr int kScaleCopies = (SC + WAVES - 1) / WAVES, kCopies = (XH * XC + NB * WC) / WAVES;      // a wave's, of a pair
     constexpr int kOutRow = 32 * NF * 4 + 16;                       // bytes of LDS, and of it a wave has 32 rows
     static_assert(XC % WAVES == 0 && WC % WAVES == 0 && BM % 64 == 0 && BN % 64 == 0, "whole copies a wave");
-    static_assert(WAVES * 32 * kOutRow <= 4 * BUFFER + 2 * SC * 1024, "the outputs' way through LDS");
-    __shared__ __align__(1024) uint8_t lds[4 * BUFFER + 2 * SC * 1024];
-    uint8_t *const scales = lds + 4 * BUFFER;
+    constexpr int kStaged = BUFFERS * (BUFFER + SC * 1024), kOut = WAVES * 32 * kOutRow;
+    __shared__ __align__(1024) uint8_t lds[kStaged > kOut ? kStaged : kOut];
+    uint8_t *const scales = lds + BUFFERS * BUFFER;
 
-    const int64_t mtiles = (a.M + BM - 1) / BM, tiles = mtiles * ((a.N + BN - 1) / BN);
-    if (nc::workgroup_id() >= tiles) return;
-    const int64_t tile = tile_of(nc::workgroup_id(), tiles);
-    const int64_t m0 = tile % mtiles * BM, n0 = tile / mtiles * BN;
-    const int lane = threadIdx.x & 63, row = lane & 31, g = lane >> 5, steps = a.steps;
+    const uint32_t mtiles = ((uint32_t)a.M + BM - 1) / BM, ntiles = ((uint32_t)a.N + BN - 1) / BN;
+    if (nc::workgroup_id() >= mtiles * ntiles) return;
+    const Tile tile = tile_of((uint32_t)nc::workgroup_id(), mtiles, ntiles);
+    const int64_t m0 = tile.m * BM, n0 = tile.n * BN;
+    const int lane = threadIdx.x & 63, row = lane & 31, g = lane >> 5, steps = a.steps, odd = steps & 1;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN * (32 * MF), wn = wave % WN * (32 * NF);      // this wave's first row of each
-    auto x_row = [&](int r) { return (uint32_t)min((int64_t)r, a.M - 1 - m0) * (uint32_t)steps; };
-    auto w_row = [&](int r) { return (uint32_t)min((int64_t)r, a.N - 1 - n0) * (uint32_t)steps; };
+    const int x_last = (int)min(a.M - 1 - m0, (int64_t)BM - 1), w_last = (int)min(a.N - 1 - n0, (int64_t)BN - 1);
+    auto x_row = [&](int r) { return (uint32_t)(min(r, x_last) * steps); };
+    auto w_row = [&](int r) { return (uint32_t)(min(r, w_last) * steps); };
     const uint8_t *xq = a.xq + (size_t)m0 * steps * (16 * BITS), *xs = a.xs + (size_t)m0 * steps * 4;
     const uint8_t *q[NB], *ws[NB];
 #pragma unroll
@@ -401,15 +394,18 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
         q[b] = a.q[b] + (size_t)n0 * steps * 64;
         ws[b] = a.ws[b] + (size_t)n0 * steps * 4;
     }
-    // This lane's part of the wave's copies: copies i * WAVES + wave of a stage, and of a group of scales.
+    // This lane's part of the wave's copies: copies i * WAVES + wave of an operand, and of a group of scales. 8-bit rows
+    // are two 128-byte ones, a step each, the halves of a block four chunks apart.
     uint32_t xat[XC / WAVES], wat[WC / WAVES];
     const uint8_t *sat[kScaleCopies];
 #pragma unroll
-    for (int i = 0; i < XC / WAVES; ++i)
-        xat[i] = x_row(X::row(lane, i * WAVES + wave)) * (16 * BITS) + X::column(lane, i * WAVES + wave);
+    for (int i = 0; i < XC / WAVES; ++i) {
+        const int c = i * WAVES + wave;
+        xat[i] = x_row(S::row(lane, c)) * (16 * BITS) + (BITS == 4 ? S::slot(lane, c) * 16 : S::column(lane, c));
+    }
 #pragma unroll
     for (int i = 0; i < WC / WAVES; ++i)
-        wat[i] = w_row(W::row(lane, i * WAVES + wave)) * 64 + W::column(lane, i * WAVES + wave);
+        wat[i] = w_row(S::row(lane, i * WAVES + wave)) * 64 + S::slot(lane, i * WAVES + wave) * 16;
 #pragma unroll
     for (int i = 0; i < kScaleCopies; ++i) {
         // (where the copies are fewer than the waves, several waves make the last one)
@@ -419,24 +415,23 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
                                : ws[NB - 1] + w_row(r - BM - BN) * 4;
     }
     const uint32_t base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t *)lds;
-    // Steps past the last are copied as the last, to keep the count of copies in flight; they are not multiplied.
-    auto copy_stage = [&](int s, int buffer) {
+    // The first of the two steps in pair p's buffer. Pairs past the last are copied as the last and not multiplied.
+    auto first_step = [&](int p) { return min(2 * p, steps - 2); };
+    // Copy i of pair p into buffer p % BUFFERS; after kCopies those of its scales, if p is even.
+    auto copy_piece = [&](int p, int buffer, int i) {
+        const int s = first_step(p);
         const uint32_t to = base + buffer * BUFFER + wave * 1024;
-        if (buffer == 0) {                                          // s % 4 == 0
-            const int first = min(s, steps - 4);                    // 16 bytes of every row are inside it
-#pragma unroll
-            for (int i = 0; i < kScaleCopies; ++i)
-                copy_to_lds_counted(sat[i] + first * 4, base + 4 * BUFFER + (s / 4 % 2 * SC + min(i * WAVES + wave, SC - 1)) * 1024);
+        if (i < XH * (XC / WAVES)) {
+            const int t = i / (XC / WAVES), c = i % (XC / WAVES);
+            copy_to_lds_counted(xq + (size_t)(s + t) * (16 * BITS) + xat[c], to + (t * XC + c * WAVES) * 1024);
+        } else if (i < kCopies) {
+            const int j = i - XH * (XC / WAVES), b = j / (WC / WAVES), c = j % (WC / WAVES);
+            copy_to_lds_counted(q[b] + (size_t)s * 64 + wat[c], to + (XH * XC + b * WC + c * WAVES) * 1024);
+        } else {                                                    // 16 bytes of every row lie inside it
+            const int c = i - kCopies;
+            copy_to_lds_counted(sat[c] + min(2 * p, steps - 4) * 4,
+                                base + BUFFERS * BUFFER + (p / 2 % BUFFERS * SC + min(c * WAVES + wave, SC - 1)) * 1024);
         }
-        s = min(s, steps - 1);
-#pragma unroll
-        for (int i = 0; i < XC / WAVES; ++i)
-            copy_to_lds_counted(xq + (size_t)s * (16 * BITS) + xat[i], to + i * WAVES * 1024);
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int i = 0; i < WC / WAVES; ++i)
-                copy_to_lds_counted(q[b] + (size_t)s * 64 + wat[i], to + (XC + b * WC + i * WAVES) * 1024);
     };
     // Half a step's operands: a lane's block g + 2 half of every row it multiplies.
     struct Half {
@@ -446,82 +441,188 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
     struct Scales {
         uint32_t x[MF], w[NB][NF];
     };
-    auto read_half = [&](Half &f, int buffer, int half) {
+    constexpr int kReads = NB * NF + MF * XH, kRows = NB * NF + MF;        // LDS reads of a half, of a step's scales
+    // Read p of half `half` of step `step` (0, 1) of a buffer. (The second step's 4-bit blocks are chunks 4 .. 7 of a row.)
+    auto read_half = [&](Half &f, int buffer, int step, int half, int p) {
         const uint8_t *from = lds + buffer * BUFFER;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int j = 0; j < NF; ++j)
-                f.w[b][j] = *reinterpret_cast<const i32x4 *>(from + (XC + b * WC) * 1024 + 32 * j * 64 +
-                                                             W::at(wn + row, g + 2 * half, 0));
-#pragma unroll
-        for (int i = 0; i < MF; ++i)
-#pragma unroll
-            for (int h = 0; h < XH; ++h)
-                f.x[i][h] = *reinterpret_cast<const i32x4 *>(from + 32 * i * (16 * BITS) + X::at(wm + row, g + 2 * half, h));
+        const int block = g + 2 * half;
+        if (p < NB * NF) {
+            f.w[p / NF][p % NF] = *reinterpret_cast<const i32x4 *>(from + (XH * XC + p / NF * WC) * 1024 + 32 * (p % NF) * 128 +
+                                                                   (S::at(wn + row, block, 0) ^ 64 * step));
+        } else {
+            const int i = (p - NB * NF) / XH, h = (p - NB * NF) % XH;
+            f.x[i][h] = *reinterpret_cast<const i32x4 *>(
+                from + 32 * i * 128 +
+                (BITS == 4 ? S::at(wm + row, block, 0) ^ 64 * step : step * XC * 1024 + S::at(wm + row, block, h)));
+        }
     };
-    auto read_scales = [&](Scales &e, int s) {
+    auto read_scales = [&](Scales &e, int s, int p) {
         s = min(s, steps - 1);
-        const uint8_t *from = scales + s / 4 % 2 * (SC * 1024) + (s - min(s & ~3, steps - 4)) * 4;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int j = 0; j < NF; ++j)
-                e.w[b][j] = *reinterpret_cast<const uint32_t *>(from + (BM + b * BN + wn + 32 * j + row) * 16);
-#pragma unroll
-        for (int i = 0; i < MF; ++i) e.x[i] = *reinterpret_cast<const uint32_t *>(from + (wm + 32 * i + row) * 16);
+        const uint8_t *from = scales + (BUFFERS == 2 ? s >> 2 & 1 : 0) * (SC * 1024) + (s - min(s & ~3, steps - 4)) * 4;
+        if (p < NB * NF) {
+            const int r = BM + p / NF * BN + wn + 32 * (p % NF) + row;
+            e.w[p / NF][p % NF] = *reinterpret_cast<const uint32_t *>(from + r * 16);
+        } else {
+            e.x[p - NB * NF] = *reinterpret_cast<const uint32_t *>(from + (wm + 32 * (p - NB * NF) + row) * 16);
+        }
     };
     f32x16 acc[NB][MF][NF] = {};
-    auto multiply = [&](const Half &f, const Scales &e, auto half) {
-        constexpr int T = decltype(half)::value;
-        // a matrix instruction picks the scale's byte itself; a conversion needs it alone
-        auto scale = [&](uint32_t e) { return BITS == 4 ? (int)(e >> (8 * g)) : (int)(e >> (8 * g + 16 * T) & 255); };
-        Block<BITS> x[MF];
+    // Half a step's products, the outputs acc[n = 8 (r / 4) + 4 (l / 32) + r % 4][m = l % 32]. `other(p)`, p < pieces, is
+    // the next half's reads and copies, spread between the products: in one place they would leave the matrix
+    // core idle, as all waves come to them at once. 4 bits: 64 values of k in one instruction, which picks a scale's
+    // byte itself.
+    auto multiply = [&](const Half &f, const Scales &e, auto half, int pieces, auto other) {
+        constexpr int OP = 2 * decltype(half)::value, products = NB * NF * MF;
+        auto wide = [](i32x4 v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); };
 #pragma unroll
-        for (int i = 0; i < MF; ++i) x[i] = x_block<BITS>(f.x[i], scale(e.x[i]));
+        for (int k = 0; k < products; ++k) {
+            const int b = k / (NF * MF), j = k / MF % NF, i = k % MF;
+            acc[b][i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                wide(f.w[b][j]), wide(f.x[i][0]), acc[b][i][j], 4, 4, OP, e.w[b][j] >> (8 * g), OP, e.x[i] >> (8 * g));
+#pragma unroll
+            for (int p = k * pieces / products; p < (k + 1) * pieces / products; ++p) other(p);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // 8 bits: four parts of 8 values a lane, each converted while the part before it is multiplied.
+    struct Part {
+        bf16x8 x[MF], w[NB][NF];
+    } part;
+    struct Powers {
+        float x[MF], w[NB][NF];
+    } powers;
+    auto take_powers = [&](const Scales &e, int half) {
+        const int shift = 8 * g + 16 * half;
+#pragma unroll
+        for (int i = 0; i < MF; ++i) powers.x[i] = power(e.x[i] >> shift & 255);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int j = 0; j < NF; ++j) {
-                const Block<BITS> w = block_of<BITS>(f.w[b][j], scale(e.w[b][j]));
-#pragma unroll
-                for (int i = 0; i < MF; ++i) acc[b][i][j] = mx_half_step<2 * T>(w, x[i], acc[b][i][j]);
-            }
+            for (int j = 0; j < NF; ++j) powers.w[b][j] = power(e.w[b][j] >> shift & 255);
     };
-    constexpr std::integral_constant<int, 0> first_half{};
-    constexpr std::integral_constant<int, 1> second_half{};
+    auto convert = [&](Part &to, const Half &f, int t, int p) {
+        if (p < NB * NF) {
+            to.w[p / NF][p % NF] = to_bf16(f.w[p / NF][p % NF][t], powers.w[p / NF][p % NF]);
+        } else {
+            const int i = p - NB * NF;
+            to.x[i] = to_bf16(f.x[i][t / 2 % XH][t % 2 * 2], f.x[i][t / 2 % XH][t % 2 * 2 + 1], powers.x[i]);
+        }
+    };
+    // Half f, whose first part is in `part`; leaves the first part of half `half` of a step of scales e, f_next, there.
+    auto multiply_converted = [&](const Half &f, const Half &f_next, const Scales &e, int half, int pieces, auto other) {
+        constexpr int products = NB * NF * MF;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            Part next;
+            if (t == 3) take_powers(e, half);
+#pragma unroll
+            for (int k = 0; k < products; ++k) {
+                const int b = k / (NF * MF), j = k / MF % NF, i = k % MF;
+                acc[b][i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(part.w[b][j], part.x[i], acc[b][i][j], 0, 0, 0);
+                // the other work in the first three parts: what it reads is converted in the fourth
+                if (t < 3) {
+                    const int at = t * products + k, of = 3 * products;
+#pragma unroll
+                    for (int p = at * pieces / of; p < (at + 1) * pieces / of; ++p) other(p);
+                }
+#pragma unroll
+                for (int p = k * kRows / products; p < (k + 1) * kRows / products; ++p)
+                    convert(next, t < 3 ? f : f_next, (t + 1) % 4, p);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            part = next;
+        }
+    };
     Half f0, f1;
     Scales e0, e1;
-    // Step s, whose first half f0 and scales e hold; leaves the next step's there and in `next`.
-    auto step = [&](int s, auto which, Scales &e, Scales &next) {
-        constexpr int U = decltype(which)::value;                   // s % 4, the step's buffer
-        // the copies that may stay in flight: those of step s + 2
-        constexpr int later = kCopies + (U == 2 ? kScaleCopies : 0);
-        read_half(f1, U, 1);
-        multiply(f0, e, first_half);
-        __builtin_amdgcn_sched_barrier(0);                          // (products may not sink past the waits)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(later) : "memory");
-        __builtin_amdgcn_s_barrier();                               // every wave's part has landed, and step s is read
-        asm volatile("" ::: "memory");
-        read_half(f0, (U + 1) % 4, 0);
-        read_scales(next, s + 1);
-        copy_stage(s + 3, (U + 3) % 4);
-        multiply(f1, e, second_half);
-        __builtin_amdgcn_sched_barrier(0);
+    constexpr std::integral_constant<int, 0> first_half{};
+    constexpr std::integral_constant<int, 1> second_half{};
+    auto product = [&](const Half &f, const Half &f_next, const Scales &e, const Scales &e_next, auto half, int pieces,
+                       auto other) {
+        if constexpr (BITS == 4) multiply(f, e, half, pieces, other);
+        else multiply_converted(f, f_next, e_next, 1 - decltype(half)::value, pieces, other);
     };
-    copy_stage(0, 0);
-    copy_stage(1, 1);
-    copy_stage(2, 2);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kCopies) : "memory");
+    // A pair's first step (f0 and e0 hold its first half and scales), and then its second's first half read.
+    auto first = [&](int p, auto which) {
+        constexpr int B = decltype(which)::value;
+        product(f0, f1, e0, e0, first_half, kReads, [&](int i) { read_half(f1, B, 0, 1, i); });
+        product(f1, f0, e0, e1, second_half, kReads + kRows, [&](int i) {
+            if (i < kReads) read_half(f0, B, 1, 0, i);
+            else read_scales(e1, first_step(p) + 1, i - kReads);
+        });
+    };
+    // The first half of step `begin` of buffer 0, step s.
+    auto begin_pair = [&](int begin, int s) {
+#pragma unroll
+        for (int i = 0; i < kReads; ++i) read_half(f0, 0, begin, 0, i);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) read_scales(e0, s, i);
+        if constexpr (BITS == 8) {
+            take_powers(e0, 0);
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) convert(part, f0, 0, i);
+        }
+    };
+    const int pairs = (steps + 1) / 2;
+    // A pair's second step (f0 and e1 hold its first half and scales); the next pair's first half read, of its second step
+    // where that is the last, odd one.
+    auto second = [&](int p, auto which) {
+        constexpr int B = decltype(which)::value;
+        product(f0, f1, e1, e1, first_half, kReads, [&](int i) { read_half(f1, B, 1, 1, i); });
+        const int begin = p + 2 == pairs ? odd : 0;
+        if constexpr (BUFFERS == 1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                           // pair p is read by every wave
+            asm volatile("" ::: "memory");
+            if (p % 2 == 1) {
+#pragma unroll
+                for (int i = kCopies; i < kCopies + kScaleCopies; ++i) copy_piece(p + 1, 0, i);
+            }
+            product(f1, f1, e1, e1, second_half, kCopies, [&](int i) { copy_piece(p + 1, 0, i); });
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                           // pair p + 1 has landed
+            asm volatile("" ::: "memory");
+            begin_pair(begin, 2 * p + 2);
+        } else {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                           // pair p + 1 has landed, pair p is read, by every wave
+            asm volatile("" ::: "memory");
+            product(f1, f0, e1, e0, second_half, kReads + kRows + kCopies + (B == 0 ? kScaleCopies : 0), [&](int i) {
+                if (i < kReads) read_half(f0, 1 - B, begin, 0, i);
+                else if (i < kReads + kRows) read_scales(e0, 2 * p + 2, i - kReads);
+                else copy_piece(p + 2, B, i - kReads - kRows);
+            });
+        }
+    };
+    auto pair = [&](int p, auto which) {
+        if (!odd || p + 1 < pairs) first(p, which);
+        else e1 = e0;
+        second(p, which);
+    };
+#pragma unroll
+    for (int i = 0; i < kCopies + kScaleCopies; ++i) copy_piece(0, 0, i);
+    if constexpr (BUFFERS == 2) {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) copy_piece(1, 1, i);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BUFFERS == 2 ? kCopies : 0) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    read_half(f0, 0, 0);
-    read_scales(e0, 0);
-    for (int s = 0; s < steps; s += 4) {
-        step(s, std::integral_constant<int, 0>{}, e0, e1);
-        if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>{}, e1, e0);
-        if (s + 2 < steps) step(s + 2, std::integral_constant<int, 2>{}, e0, e1);
-        if (s + 3 < steps) step(s + 3, std::integral_constant<int, 3>{}, e1, e0);
+    begin_pair(0, 0);
+    if constexpr (BUFFERS == 2) {
+        for (int p = 0; p < pairs; p += 2) {
+            pair(p, std::integral_constant<int, 0>{});
+            if (p + 1 < pairs) pair(p + 1, std::integral_constant<int, 1>{});
+        }
+    } else {
+        for (int p = 0; p < pairs - odd; ++p) {
+            first(p, std::integral_constant<int, 0>{});
+            second(p, std::integral_constant<int, 0>{});
+        }
+        if (odd) {                                                  // f0 and e0 hold the last step's first half and scales
+            product(f0, f1, e0, e0, first_half, kReads, [&](int i) { read_half(f1, 0, 1, 1, i); });
+            product(f1, f1, e0, e0, second_half, 0, [](int) {});
+        }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
@@ -532,7 +633,7 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
             for (int j = 0; j < NF; ++j) asm volatile("" : "+v"(acc[b][i][j]));
     __syncthreads();                                   // the last copies have landed and the last reads are done
     uint8_t *const mine = lds + wave * (32 * kOutRow);
-    constexpr int kAcross = 8 * NF, kRows = 64 / kAcross;           // lanes a row of 32 NF outputs, rows at a time
+    constexpr int kAcross = 8 * NF, kDown = 64 / kAcross;           // lanes a row of 32 NF outputs, rows at a time
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
 #pragma unroll
@@ -548,20 +649,20 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
             }
         asm volatile("" ::: "memory");                 // (a wave's LDS accesses are in order)
         const int64_t n = n0 + wn + lane % kAcross * 4;
-        f32x4 v[32 / kRows];
+        f32x4 v[32 / kDown];
 #pragma unroll
-        for (int k = 0; k < 32 / kRows; ++k)
-            v[k] = *reinterpret_cast<const f32x4 *>(mine + (k * kRows + lane / kAcross) * kOutRow + lane % kAcross * 16);
+        for (int k = 0; k < 32 / kDown; ++k)
+            v[k] = *reinterpret_cast<const f32x4 *>(mine + (k * kDown + lane / kAcross) * kOutRow + lane % kAcross * 16);
         asm volatile("" ::: "memory");
-        finish<NB, 32 / kRows>(a, m0 + wm + 32 * i + lane / kAcross, kRows, n, v);
+        finish<NB, 32 / kDown>(a, m0 + wm + 32 * i + lane / kAcross, kDown, n, v);
     }
 }
 
-template <int BITS, int NB, int WM, int WN, int MF, int NF>
+template <int BITS, int NB, int WM, int WN, int MF, int NF, int BUFFERS>
 int32_t launch_tile(const MxArgs &a) {
     constexpr int BM = 32 * MF * WM, BN = 32 * NF * WN;
     const int64_t tiles = (a.M + BM - 1) / BM * ((a.N + BN - 1) / BN);
-    hipLaunchKernelGGL((mx_tile<BITS, NB, WM, WN, MF, NF>), nc::grid_of(tiles), dim3(WM * WN * 64), 0, nc::stream(), a);
+    hipLaunchKernelGGL((mx_tile<BITS, NB, WM, WN, MF, NF, BUFFERS>), nc::grid_of(tiles), dim3(WM * WN * 64), 0, nc::stream(), a);
     return nc::launched("mx_tile");
 }
 
@@ -572,18 +673,18 @@ int32_t launch(const MxArgs &a) {
         case nc::MxTile::kRow: return launch_split<BITS, NB, 1, 1, 4, 2>(a);
         case nc::MxTile::kLongRow: return launch_split<BITS, NB, 1, 1, 8, 2>(a);
         case nc::MxTile::kSplit: return launch_split<BITS, NB, 2, 2, 4, NB == 1 ? 2 : 1>(a);
-        case nc::MxTile::kSmall: return launch_tile<BITS, NB, 2, 2, 1, 1>(a);
+        case nc::MxTile::kSmall: return launch_tile<BITS, NB, 2, 2, 1, 1, 1>(a);
         default:
-            if constexpr (BITS == 4) return launch_tile<BITS, NB, 2, 4, 4, NB == 1 ? 2 : 1>(a);
-            else if constexpr (NB == 1) return launch_tile<BITS, NB, 2, 4, 2, 2>(a);
-            else return launch_tile<BITS, NB, 2, 2, 2, 1>(a);
+            if constexpr (BITS == 4) return launch_tile<BITS, NB, 2, 4, 4, NB == 1 ? 2 : 1, 2>(a);
+            else if constexpr (NB == 1) return launch_tile<BITS, NB, 2, 4, 2, 2, 2>(a);
+            else return launch_tile<BITS, NB, 2, 4, 2, 1, 2>(a);
     }
 }
 
-// Shapes whose outputs are fewer than 2^40 (a terabyte of float32 is 2^38) and whose rows a tile addresses in 32 bits.
+// Shapes whose outputs are fewer than 2^39 (two terabytes of float32; tiles of 16 x 16 are counted in 32 bits) and whose rows a tile addresses in 32 bits.
 bool mx_matmul_shape(const int64_t *s) {
     return s[0] >= 0 && s[1] > 0 && s[2] > 0 && s[0] < (1 << 26) && s[1] < (1 << 26) && s[2] <= (1 << 24) &&
-           s[0] * s[1] < (int64_t)1 << 40;
+           s[0] * s[1] < (int64_t)1 << 39;
 }
 
 }  // namespace
