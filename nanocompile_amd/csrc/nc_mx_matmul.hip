@@ -355,34 +355,44 @@ __device__ __forceinline__ void copy_to_lds_counted(const uint8_t *from, uint32_
                  "s"(__builtin_amdgcn_readfirstlane(to)) : "m0", "memory");
 }
 
-// Many outputs: a workgroup of WM x WN waves takes 32 MF WM rows of x by 32 NF WN weight rows (of each weight), each wave
-// 32 MF x 32 NF of them. Operands are staged in LDS two steps at a time, in two buffers: 4-bit rows are copied 128
-// bytes at a time, as whole lines of the cache come twice as fast as halves (measured: 33 against 16 TB/s). A wave
-// reads half a step's operands into registers while it multiplies the half before. One barrier a pair of steps, before
-// its last half: by then the next pair has landed and this one is read, so the copies of the pair after next start,
-// with two steps to land. Where the steps are odd the last is the second of a pair whose first is not multiplied again.
+// Many outputs: a workgroup of WM x WN waves takes 32 MF WM rows of x by 32 NF WN weight rows (of each weight), each
+// wave 32 MF x 32 NF of them. Operands are staged in LDS two steps at a time: 4-bit rows are copied 128 bytes at a time,
+// as whole lines of the cache come twice as fast as halves (measured: 33 against 16 TB/s). A wave reads half a step's
+// operands into registers while it multiplies the half before.
+// With two buffers there is one barrier a pair of steps, before its last half: by then the next pair has landed and this
+// one is read, so the copies of the pair after next start, with two steps to land. With one the next pair's copies
+// start at that barrier and have landed at another, half a step later: other workgroups, of which a CU takes twice as
+// many, fill the wait. Where the steps are odd the last is the second of a pair whose first is not multiplied again.
 // The scales come four steps at a time, 16 bytes a row, with the pairs 0, 2, 4 ... The outputs go through LDS, a wave's
 // 32 rows at a time, so that whole lines are written (a lane's own outputs are 16 bytes of a row: 4096 x 8192 x 8192
-// took 255 us so, 140 of them without the stores). Needs four steps.
-template <int BITS, int NB, int WM, int WN, int MF, int NF, int BUFFERS>
-__global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
+// took 255 us so, 140 of them without the stores).
+// With WK > 1 the tile is one wave's, and WK waves have the whole of it and a part of k each, with stages of their own
+// and so without barriers; their sums are added in the order of the waves. For the shapes whose tiles are few and k
+// long: 512 x 896 x 4864 in 4 bits 6.5 us (8.7 with 64 x 64 by four waves), 128 x 4096 x 4096 in 8 bits 8.7 (11.4 with
+// mx_split). Needs four steps.
+template <int BITS, int NB, int WM, int WN, int MF, int NF, int BUFFERS, int WK>
+__global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
+    static_assert(WK == 1 || WM * WN == 1, "k is split over waves that have the whole tile each");
     using S = Stage<128, 2>;
     constexpr int WAVES = WM * WN, BM = 32 * MF * WM, BN = 32 * NF * WN, XH = BITS / 4;
-    constexpr int XC = BM / 8, WC = BN / 8, SC = (BM + NB * BN) / 64;       // copies of 128-byte rows; of a group of scales
+    constexpr int XC = BM / 8, WC = BN / 8, SC = (BM + NB * BN + 63) / 64;  // copies of 128-byte rows; of a group of scales
     constexpr int BUFFER = (XH * XC + NB * WC) * 1024;
     constexpr int kScaleCopies = (SC + WAVES - 1) / WAVES, kCopies = (XH * XC + NB * WC) / WAVES;      // a wave's, of a pair
     constexpr int kOutRow = 32 * NF * 4 + 16;                       // bytes of LDS, and of it a wave has 32 rows
-    static_assert(XC % WAVES == 0 && WC % WAVES == 0 && BM % 64 == 0 && BN % 64 == 0, "whole copies a wave");
-    constexpr int kStaged = BUFFERS * (BUFFER + SC * 1024), kOut = WAVES * 32 * kOutRow;
-    __shared__ __align__(1024) uint8_t lds[kStaged > kOut ? kStaged : kOut];
+    static_assert(XC % WAVES == 0 && WC % WAVES == 0, "whole copies a wave");
+    constexpr int kStaged = BUFFERS * (BUFFER + SC * 1024), kOut = WAVES * (WK == 1 ? 1 : NB) * 32 * kOutRow;
+    constexpr int kShare = kStaged > kOut ? kStaged : kOut;
+    __shared__ __align__(1024) uint8_t all_lds[WK * kShare];
+    const int member = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = WK == 1 ? member : 0, part_of_k = WK == 1 ? 0 : member;
+    uint8_t *const lds = all_lds + part_of_k * kShare;
     uint8_t *const scales = lds + BUFFERS * BUFFER;
 
     const uint32_t mtiles = ((uint32_t)a.M + BM - 1) / BM, ntiles = ((uint32_t)a.N + BN - 1) / BN;
     if (nc::workgroup_id() >= mtiles * ntiles) return;
     const Tile tile = tile_of((uint32_t)nc::workgroup_id(), mtiles, ntiles);
     const int64_t m0 = tile.m * BM, n0 = tile.n * BN;
-    const int lane = threadIdx.x & 63, row = lane & 31, g = lane >> 5, steps = a.steps, odd = steps & 1;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, row = lane & 31, g = lane >> 5, steps = a.steps;
     const int wm = wave / WN * (32 * MF), wn = wave % WN * (32 * NF);      // this wave's first row of each
     const int x_last = (int)min(a.M - 1 - m0, (int64_t)BM - 1), w_last = (int)min(a.N - 1 - n0, (int64_t)BN - 1);
     auto x_row = [&](int r) { return (uint32_t)(min(r, x_last) * steps); };
@@ -415,23 +425,35 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
                                : ws[NB - 1] + w_row(r - BM - BN) * 4;
     }
     const uint32_t base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    // This wave's pairs of steps, and whether its last is the odd step alone.
+    const int pairs = (steps + 1) / 2, share = (pairs + WK - 1) / WK;
+    const int p_begin = part_of_k * share, p_end = min(pairs, p_begin + share), odd = p_end == pairs ? steps & 1 : 0;
+    // Waves that share a stage wait for each other; those with a part of k each have none to wait for.
+    auto meet = [] {
+        if constexpr (WAVES > 1) __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
     // The first of the two steps in pair p's buffer. Pairs past the last are copied as the last and not multiplied.
     auto first_step = [&](int p) { return min(2 * p, steps - 2); };
-    // Copy i of pair p into buffer p % BUFFERS; after kCopies those of its scales, if p is even.
+    // Copy i of pair p into a buffer.
     auto copy_piece = [&](int p, int buffer, int i) {
         const int s = first_step(p);
         const uint32_t to = base + buffer * BUFFER + wave * 1024;
         if (i < XH * (XC / WAVES)) {
             const int t = i / (XC / WAVES), c = i % (XC / WAVES);
             copy_to_lds_counted(xq + (size_t)(s + t) * (16 * BITS) + xat[c], to + (t * XC + c * WAVES) * 1024);
-        } else if (i < kCopies) {
+        } else {
             const int j = i - XH * (XC / WAVES), b = j / (WC / WAVES), c = j % (WC / WAVES);
             copy_to_lds_counted(q[b] + (size_t)s * 64 + wat[c], to + (XH * XC + b * WC + c * WAVES) * 1024);
-        } else {                                                    // 16 bytes of every row lie inside it
-            const int c = i - kCopies;
-            copy_to_lds_counted(sat[c] + min(2 * p, steps - 4) * 4,
-                                base + BUFFERS * BUFFER + (p / 2 % BUFFERS * SC + min(c * WAVES + wave, SC - 1)) * 1024);
         }
+    };
+    // The scales of the four steps that pair p is of: 16 bytes that lie inside every row.
+    auto copy_scales = [&](int p) {
+        const int first = min(p / 2 * 4, steps - 4);
+#pragma unroll
+        for (int i = 0; i < kScaleCopies; ++i)
+            copy_to_lds_counted(sat[i] + first * 4,
+                                base + BUFFERS * BUFFER + (p / 2 % BUFFERS * SC + min(i * WAVES + wave, SC - 1)) * 1024);
     };
     // Half a step's operands: a lane's block g + 2 half of every row it multiplies.
     struct Half {
@@ -563,65 +585,64 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
             for (int i = 0; i < kRows; ++i) convert(part, f0, 0, i);
         }
     };
-    const int pairs = (steps + 1) / 2;
     // A pair's second step (f0 and e1 hold its first half and scales); the next pair's first half read, of its second step
     // where that is the last, odd one.
     auto second = [&](int p, auto which) {
         constexpr int B = decltype(which)::value;
         product(f0, f1, e1, e1, first_half, kReads, [&](int i) { read_half(f1, B, 1, 1, i); });
-        const int begin = p + 2 == pairs ? odd : 0;
+        const int begin = p + 2 == p_end ? odd : 0;
         if constexpr (BUFFERS == 1) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();                           // pair p is read by every wave
-            asm volatile("" ::: "memory");
-            if (p % 2 == 1) {
-#pragma unroll
-                for (int i = kCopies; i < kCopies + kScaleCopies; ++i) copy_piece(p + 1, 0, i);
-            }
+            meet();                                                 // pair p is read by every wave
+            if (p % 2 == 1) copy_scales(p + 1);
             product(f1, f1, e1, e1, second_half, kCopies, [&](int i) { copy_piece(p + 1, 0, i); });
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();                           // pair p + 1 has landed
-            asm volatile("" ::: "memory");
+            meet();                                                 // pair p + 1 has landed
             begin_pair(begin, 2 * p + 2);
         } else {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();                           // pair p + 1 has landed, pair p is read, by every wave
-            asm volatile("" ::: "memory");
-            product(f1, f0, e1, e0, second_half, kReads + kRows + kCopies + (B == 0 ? kScaleCopies : 0), [&](int i) {
+            meet();                                                 // pair p + 1 has landed, pair p is read, by every wave
+            product(f1, f0, e1, e0, second_half, kReads + kRows + kCopies, [&](int i) {
                 if (i < kReads) read_half(f0, 1 - B, begin, 0, i);
                 else if (i < kReads + kRows) read_scales(e0, 2 * p + 2, i - kReads);
                 else copy_piece(p + 2, B, i - kReads - kRows);
             });
+            if (p % 2 == 0) copy_scales(p + 2);
         }
     };
     auto pair = [&](int p, auto which) {
-        if (!odd || p + 1 < pairs) first(p, which);
+        if (!odd || p + 1 < p_end) first(p, which);
         else e1 = e0;
         second(p, which);
     };
+    if (WK == 1 || p_begin < p_end) {
+        copy_scales(p_begin);
 #pragma unroll
-    for (int i = 0; i < kCopies + kScaleCopies; ++i) copy_piece(0, 0, i);
-    if constexpr (BUFFERS == 2) {
+        for (int i = 0; i < kCopies; ++i) copy_piece(p_begin, 0, i);
+        if constexpr (BUFFERS == 2) {
+            if (p_begin % 2 == 1) copy_scales(p_begin + 1);
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) copy_piece(1, 1, i);
-    }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BUFFERS == 2 ? kCopies : 0) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    begin_pair(0, 0);
-    if constexpr (BUFFERS == 2) {
-        for (int p = 0; p < pairs; p += 2) {
-            pair(p, std::integral_constant<int, 0>{});
-            if (p + 1 < pairs) pair(p + 1, std::integral_constant<int, 1>{});
+            for (int i = 0; i < kCopies; ++i) copy_piece(p_begin + 1, 1, i);
         }
-    } else {
-        for (int p = 0; p < pairs - odd; ++p) {
-            first(p, std::integral_constant<int, 0>{});
-            second(p, std::integral_constant<int, 0>{});
-        }
-        if (odd) {                                                  // f0 and e0 hold the last step's first half and scales
-            product(f0, f1, e0, e0, first_half, kReads, [&](int i) { read_half(f1, 0, 1, 1, i); });
-            product(f1, f1, e0, e0, second_half, 0, [](int) {});
+        // (the second pair's scales may be waited for too)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BUFFERS == 2 ? kCopies : 0) : "memory");
+        meet();
+        const int alone = odd && p_begin + 1 == p_end;              // nothing but the odd step
+        begin_pair(alone, 2 * p_begin);
+        if constexpr (BUFFERS == 2) {
+            for (int p = p_begin; p < p_end; p += 2) {
+                pair(p, std::integral_constant<int, 0>{});
+                if (p + 1 < p_end) pair(p + 1, std::integral_constant<int, 1>{});
+            }
+        } else {
+            for (int p = p_begin; p < p_end - odd; ++p) {
+                first(p, std::integral_constant<int, 0>{});
+                second(p, std::integral_constant<int, 0>{});
+            }
+            if (odd) {                                              // f0 and e0 hold the last step's first half and scales
+                product(f0, f1, e0, e0, first_half, kReads, [&](int i) { read_half(f1, 0, 1, 1, i); });
+                product(f1, f1, e0, e0, second_half, 0, [](int) {});
+            }
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -632,8 +653,39 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
 #pragma unroll
             for (int j = 0; j < NF; ++j) asm volatile("" : "+v"(acc[b][i][j]));
     __syncthreads();                                   // the last copies have landed and the last reads are done
-    uint8_t *const mine = lds + wave * (32 * kOutRow);
     constexpr int kAcross = 8 * NF, kDown = 64 / kAcross;           // lanes a row of 32 NF outputs, rows at a time
+    if constexpr (WK > 1) {
+        // every wave's sums side by side, then a share of the rows each, added in the order of the waves
+        constexpr int kAll = 32 / kDown, kMine = (kAll + WK - 1) / WK;
+        static_assert(MF == 1 && kAll % kMine == 0, "32 rows of outputs, whole shares of them");
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    *reinterpret_cast<f32x4 *>(lds + (b * 32 + row) * kOutRow + (32 * j + 8 * r + 4 * g) * 4) =
+                        f32x4{acc[b][0][j][4 * r], acc[b][0][j][4 * r + 1], acc[b][0][j][4 * r + 2], acc[b][0][j][4 * r + 3]};
+        __syncthreads();
+        if (part_of_k * kMine >= kAll) return;
+        const int down = part_of_k * (kMine * kDown) + lane / kAcross;
+        f32x4 v[kMine];
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            f32x4 sum[NB] = {};
+#pragma unroll
+            for (int w = 0; w < WK; ++w)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    sum[b] += *reinterpret_cast<const f32x4 *>(all_lds + w * kShare + (b * 32 + down + k * kDown) * kOutRow +
+                                                               lane % kAcross * 16);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[k][c] = NB == 1 ? sum[0][c] : silu_times(sum[0][c], sum[NB - 1][c]);
+        }
+        finish<NB, kMine>(a, m0 + down, kDown, n0 + lane % kAcross * 4, v);
+        return;
+    }
+    uint8_t *const mine = lds + wave * (32 * kOutRow);
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
 #pragma unroll
@@ -658,30 +710,35 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile(MxArgs a) {
     }
 }
 
-template <int BITS, int NB, int WM, int WN, int MF, int NF, int BUFFERS>
+template <int BITS, int NB, int WM, int WN, int MF, int NF, int BUFFERS, int WK = 1>
 int32_t launch_tile(const MxArgs &a) {
     constexpr int BM = 32 * MF * WM, BN = 32 * NF * WN;
     const int64_t tiles = (a.M + BM - 1) / BM * ((a.N + BN - 1) / BN);
-    hipLaunchKernelGGL((mx_tile<BITS, NB, WM, WN, MF, NF, BUFFERS>), nc::grid_of(tiles), dim3(WM * WN * 64), 0, nc::stream(), a);
+    hipLaunchKernelGGL((mx_tile<BITS, NB, WM, WN, MF, NF, BUFFERS, WK>), nc::grid_of(tiles), dim3(WM * WN * WK * 64), 0,
+                       nc::stream(), a);
     return nc::launched("mx_tile");
 }
 
 template <int BITS, int NB>
 int32_t launch(const MxArgs &a) {
-    const nc::MxTile tile = nc::mx_tile(a.M, a.N, a.steps, BITS, NB);
-    switch (tile) {
+    switch (nc::mx_tile(a.M, a.N, a.steps, BITS, NB)) {
         case nc::MxTile::kRow: return launch_split<BITS, NB, 1, 1, 4, 2>(a);
         case nc::MxTile::kLongRow: return launch_split<BITS, NB, 1, 1, 8, 2>(a);
         case nc::MxTile::kSplit: return launch_split<BITS, NB, 2, 2, 4, NB == 1 ? 2 : 1>(a);
+        case nc::MxTile::kJoined:
+            return launch_tile<BITS, NB, 1, 1, 1, BITS == 8 && NB == 1 ? 2 : 1, BITS == 4 && NB == 1 ? 1 : 2, 4>(a);
+        case nc::MxTile::kDeep: return launch_tile<BITS, NB, 2, 2, 1, 1, 2>(a);
+        case nc::MxTile::kMedium:
+            if constexpr (NB == 1) return launch_tile<BITS, NB, 2, 2, BITS == 4 ? 2 : 1, 2, 2>(a);
+            [[fallthrough]];                                        // (no pair has it)
         case nc::MxTile::kSmall: return launch_tile<BITS, NB, 2, 2, 1, 1, 1>(a);
-        default:
-            if constexpr (BITS == 4) return launch_tile<BITS, NB, 2, 4, 4, NB == 1 ? 2 : 1, 2>(a);
-            else if constexpr (NB == 1) return launch_tile<BITS, NB, 2, 4, 2, 2, 2>(a);
-            else return launch_tile<BITS, NB, 2, 4, 2, 1, 2>(a);
+        case nc::MxTile::kLarge: return launch_tile<BITS, NB, 2, 4, BITS == 4 ? 4 : 2, NB == 1 ? 2 : 1, 2>(a);
     }
+    return NC_BAD_ARGS;
 }
 
-// Shapes whose outputs are fewer than 2^39 (two terabytes of float32; tiles of 16 x 16 are counted in 32 bits) and whose rows a tile addresses in 32 bits.
+// Shapes whose outputs are fewer than 2^39 (two terabytes of float32; tiles of 16 x 16 are counted in 32 bits) and
+// whose rows a tile addresses in 32 bits.
 bool mx_matmul_shape(const int64_t *s) {
     return s[0] >= 0 && s[1] > 0 && s[2] > 0 && s[0] < (1 << 26) && s[1] < (1 << 26) && s[2] <= (1 << 24) &&
            s[0] * s[1] < (int64_t)1 << 39;

@@ -176,14 +176,48 @@ constexpr int prefill_rows(int64_t M, int64_t heads, int64_t kv_heads, int64_t k
     return group <= 4 && (M + 3) / 4 * ((keys + 63) / 64) * heads <= 1200 ? 4 : 0;
 }
 
-// The kernel of a microscaled product of M rows by N weight rows over `steps` of 128 values of k (nc_mx_matmul.hip).
-enum class MxTile { kRow, kLongRow, kSplit, kSmall, kLarge };
+// The kernel of a microscaled product of M rows by N weight rows, `weights` of them for each output, over `steps` of
+// 128 values of k, the activations of `bits` (nc_mx_matmul.hip has the kernels). The more outputs, the larger a
+// workgroup's tile, as the operands are then read less often; the fewer, the more waves share one tile's k, as the
+// chip would stay empty:
+//   kRow, kLongRow  16 x 16 outputs, k over 4 or 8 waves that each copy their rows by themselves
+//   kSplit          32 x 32, k over 4 waves of that kind; the only one for fewer than four steps and many outputs
+//   kJoined         32 x 32 (x 64 for 8 bits by one weight), k over 4 waves with the larger tiles' pipeline
+//   kSmall, kDeep   64 x 64 over 4 waves, two steps' operands in LDS or four
+//   kMedium         128 x 128 (64 x 128 for 8 bits), of one weight
+//   kLarge          256 x 256 (128 x 256 for 8 bits), half as wide for a pair
+// Both sides of each border, us (bits/weights: M x N x K):
+//   kRow / kLongRow   4/1: 2 x 4864 x 896 2.6 / 3.0, 2 x 8192 x 8192 7.3 / 7.8, 3 x 726 x 6801 4.2 / 3.9;
+//                     8/1: 13 x 4096 x 4096 4.8 / 4.0, 9 x 1305 x 4987 4.8 / 3.9; 8/2: 3 x 2048 x 8192 10.7 / 7.5
+//   kRow / kSplit     4/1: 76 x 1152 x 896 2.7 / 3.0, 199 x 918 x 287 2.9 / 2.8; 8/1: 250 x 896 x 896 3.9 / 3.6;
+//                     4/2: 58 x 4864 x 896 4.1 / 5.0; 8/2: 40 x 4864 x 896 4.5 / 5.8, 342 x 1439 x 1285 9.8 / 7.7
+//   kRow / kJoined    4/1: 105 x 896 x 4864 4.5 / 4.9, 146 x 896 x 4864 6.0 / 5.0; 8/1: 163 x 896 x 4864 7.7 / 9.2,
+//                     29 x 8192 x 8192 16.9 / 12.3; 4/2: 271 x 739 x 4251 12.1 / 7.1; 8/2: 53 x 3195 x 5597 15.1 / 11.1
+//   kSplit / kJoined  4/1: 2021 x 161 x 1104 3.9 / 4.0, 134 x 4096 x 4096 11.5 / 8.0; 8/1: 455 x 2103 x 1397 8.4 / 10.2,
+//                     343 x 2048 x 8192 25.2 / 23.0
+//   kJoined / kDeep   8/2: 1076 x 693 x 3214 21.9 / 16.2; 4/2: 190 x 3139 x 2592 15.5 / 10.2
+//   kSmall / kDeep    4/1: 294 x 16000 x 1024 10.5 / 11.2, 2162 x 896 x 4864 17.4 / 14.8; 4/2: 99 x 4864 x 896 5.4 / 5.2
+//   kSmall / kMedium  4/1: 442 x 8192 x 8192 36.1 / 29.9; 8/1: 789 x 4096 x 4096 37.8 / 30.7
+//   kDeep / kMedium   4/1: 368 x 8192 x 2048 10.3 / 11.4, 923 x 8192 x 2048 20.9 / 16.6
+//   kMedium / kLarge  4/1: 923 x 8192 x 2048 16.6 / 20.7, 1960 x 8192 x 2048 30.2 / 26.0; 8/1: 1270 x 4988 x 4760 69 / 54
+//   kSmall / kLarge   4/2: 465 x 4864 x 896 8.6 / 13.9, 3887 x 4096 x 4096 110 / 71; 8/2: 993 x 4864 x 896 21.6 / 28.7,
+//                     1867 x 8192 x 8192 432 / 372
+enum class MxTile { kRow, kLongRow, kSplit, kJoined, kSmall, kDeep, kMedium, kLarge };
 
 constexpr MxTile mx_tile(int64_t M, int64_t N, int64_t steps, int bits, int weights) {
-    if (M <= 16) return steps >= 16 ? MxTile::kLongRow : MxTile::kRow;
-    const int64_t tiles = (M + 63) / 64 * ((N + 63) / 64) * weights;
-    if (steps < 4 || tiles < 256) return MxTile::kSplit;
-    return tiles < 4096 ? MxTile::kSmall : MxTile::kLarge;
+    auto tiles = [&](int64_t rows, int64_t columns) { return (M + rows - 1) / rows * ((N + columns - 1) / columns); };
+    const int64_t t32 = tiles(32, 32), work = tiles(64, 64) * weights;
+    const bool few = steps < 20 ? t32 < 170 * weights : tiles(32, bits == 8 && weights == 1 ? 64 : 32) < 110;
+    if (M <= 16 || few) return steps >= 10 && t32 <= 130 ? MxTile::kLongRow : MxTile::kRow;
+    if (steps < 4) return MxTile::kSplit;
+    if (work < 300) return steps >= 12 ? MxTile::kJoined : MxTile::kSplit;
+    // kLarge has one workgroup on each of the 256 CUs: where its last round of them would be mostly empty, or the rows
+    // past M and N much of its work, smaller ones are quicker
+    const int64_t rows = bits == 4 ? 256 : 128, columns = 256 / weights;
+    const int64_t places = (tiles(rows, columns) + 255) / 256 * 256 * rows * columns;
+    if (steps >= 8 && M * N >= places / 5 * 3) return MxTile::kLarge;
+    if (weights == 1 && work >= 800 && steps >= 12) return MxTile::kMedium;
+    return steps >= 8 && work < 800 ? MxTile::kDeep : MxTile::kSmall;
 }
 
 }  // namespace nc

@@ -250,14 +250,25 @@ WIDE = [(1100, 1000, 513), (1030, 1024, 896), (1025, 1090, 768), (1089, 1030, 51
         (4100, 4130, 520), (4097, 4099, 896), (4128, 4100, 1024)]
 
 
+# few outputs and long k, whose k is split over four waves in pairs of steps: 12, 13, 17, 19, 20, 38 steps
+LONG = [(330, 1000, 1500), (333, 1001, 1537), (321, 1003, 2176), (350, 997, 2305), (322, 1024, 2560), (352, 1025, 4864)]
+
+# the same with short k
+SHORT = [(330, 1001, 1100), (701, 700, 300), (355, 1003, 600)]
+
+# many outputs again: 64 x 64 tiles of eight steps and more, the larger ones, their borders ragged
+TILES = [(1300, 1000, 1024), (1281, 1025, 1100), (1300, 1030, 1153), (1281, 1000, 513), (1800, 1900, 1537), (1793, 1921, 2560),
+         (3200, 3201, 1100), (3203, 3200, 1024), (3210, 3210, 1300)]
+
+
 @pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("m,n,k", SHAPES + WIDE)
+@pytest.mark.parametrize("m,n,k", SHAPES + WIDE + LONG + SHORT + TILES)
 def test_matmul(gpu, m, n, k, bits):
     check_matmul(m, n, k, bits)
 
 
 @pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("m,n,k", SHAPES + WIDE)
+@pytest.mark.parametrize("m,n,k", SHAPES + WIDE + LONG + SHORT + TILES)
 def test_swiglu(gpu, m, n, k, bits):
     check_swiglu(m, n, k, bits)
 
