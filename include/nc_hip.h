@@ -171,7 +171,8 @@ int32_t nc_matmul_i8_token_swiglu(void **p, const int64_t *s);
  * is padded with zeros to steps = ceil(K / 128) times 128: codes u8[rows, steps * 16 * bits]
  * (two 4-bit elements a byte, the lower index in the low bits), scales
  * u8[rows, steps * 4]. Codes lie on 16-byte boundaries, scales on 4-byte ones
- * (others are refused); float32 operands on any boundary of a float. */
+ * (others are refused); float32 operands on any boundary of a float. Rows and
+ * columns are fewer than 2^26. */
 
 /* Rows to MX: a block's scale puts its largest value into the elements' top
  * binade (floor(log2(max|x|)) - 2 or - 8, at least -127), each value times the inverse
@@ -199,9 +200,9 @@ int32_t nc_dequantize_mx(void **p, const int64_t *s);
 int32_t nc_add_rms_norm_quant(void **p, const int64_t *s);
 
 /* y = x @ w.T of MX activations (of 4 or 8 bits) and MX 4-bit weights, added in
- * float32 on the scaled matrix cores, then + bias, then residual + y. A row that
- * holds a NaN scale gives NaN outputs; y may be the residual, and overlaps no
- * other operand.
+ * float32 on the matrix cores, then + bias, then residual + y. A row of x or of
+ * the weights that holds a NaN scale gives NaN outputs; y may be the residual, and
+ * overlaps no other operand.
  * p: [y f32[M,N], xq codes, xs scales, q codes of N rows, scales of N rows,
  *     bias f32[N] or NULL, residual f32[M,N] or NULL];
  * s: [M, N, K, bits of xq (4 or 8)] (M * N < 2^39, K at most 2^24) */

@@ -22,40 +22,38 @@ constexpr int kMxBlock = 32, kMxPad = 128, kMxNan = 255;
 
 inline __host__ __device__ int64_t mx_padded(int64_t k) { return (k + kMxPad - 1) / kMxPad * kMxPad; }
 
-// 16 and 8 bytes of floats at any address of a float (a row of an odd width starts at one): global memory
-// takes wide loads and stores on 4-byte boundaries.
+// 16 bytes of floats at any address of a float (a row of an odd width starts at one): global memory takes wide
+// loads and stores on 4-byte boundaries.
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// 8 values from p of which the first `valid` (<= 0: none) are a row's: zeros for the others, which are not read.
-__device__ __forceinline__ void load8(float (&v)[8], const float *p, int valid) {
-    if (valid >= 8) {
-        const f32x4 a = *reinterpret_cast<const f32x4_any *>(p), b = *reinterpret_cast<const f32x4_any *>(p + 4);
+// 4 values from p of which the first `valid` (<= 0: none) are a row's: zeros for the others, which are not read.
+__device__ __forceinline__ f32x4 load4(const float *p, int valid) {
+    if (valid >= 4) return *reinterpret_cast<const f32x4_any *>(p);
+    f32x4 v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < valid ? p[j] : 0.0f;
-    }
+    for (int j = 0; j < 4; ++j) v[j] = j < valid ? p[j] : 0.0f;
+    return v;
 }
 
-__device__ __forceinline__ void store8(float *p, const float (&v)[8], int valid) {
-    if (valid >= 8) {
-        *reinterpret_cast<f32x4_any *>(p) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4_any *>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+// KEPT: through the caches as any store, otherwise past them (the last values of a row that are not four excepted).
+template <bool KEPT = true>
+__device__ __forceinline__ void store4(float *p, f32x4 v, int valid) {
+    if (valid >= 4) {
+        if constexpr (KEPT) *reinterpret_cast<f32x4_any *>(p) = v;
+        else __builtin_nontemporal_store(v, reinterpret_cast<f32x4_any *>(p));
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 3; ++j)
             if (j < valid) p[j] = v[j];
     }
 }
 
 // |v| as bits: ordered as the values, an infinity and then the NaNs above them.
-__device__ __forceinline__ int32_t magnitude_bits(const float (&v)[8]) {
+__device__ __forceinline__ int32_t magnitude_bits(f32x4 v) {
     int32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_int(v[j]) & 0x7fffffff);
+    for (int j = 0; j < 4; ++j) m = max(m, __float_as_int(v[j]) & 0x7fffffff);
     return m;
 }
 
@@ -66,56 +64,44 @@ __device__ __forceinline__ int mx_scale(int32_t magnitude) {
     return magnitude >= 0x7f800000 ? kMxNan : max((magnitude >> 23) - (BITS == 4 ? 2 : 8), 0);
 }
 
-// 8 consecutive values of a block of the given scale to elements: 4 bytes, or 8 (the second word 0 in 4 bits).
+// 4 consecutive values of a block of the given scale to elements, in the low 16 bits or all 32.
 // The conversions round to nearest even and keep 4-bit values past 6 at 6 (checked against every rounding
 // border); past 464 the 8-bit one would give NaN, hence the clamp. The inverse of a scale 0 .. 252 is the
 // normal float of exponent 254 - scale.
 template <int BITS>
-__device__ __forceinline__ u32x2 mx_encode(const float (&v)[8], int scale) {
+__device__ __forceinline__ uint32_t mx_encode(f32x4 v, int scale) {
     const float inverse = __uint_as_float((uint32_t)(254 - scale) << 23);
-    float t[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = scale == kMxNan ? 0.0f : __fmul_rn(v[j], inverse);
-    u32x2 out = {0u, 0u};
+    for (int j = 0; j < 4; ++j) v[j] = scale == kMxNan ? 0.0f : __fmul_rn(v[j], inverse);
     if constexpr (BITS == 4) {
-        uint32_t w = 0;
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[0], t[1], 1.0f, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[2], t[3], 1.0f, 1);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[4], t[5], 1.0f, 2);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[6], t[7], 1.0f, 3);
-        out[0] = w;
+        const uint32_t low = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], 1.0f, 0);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(low, v[2], v[3], 1.0f, 1);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = __builtin_amdgcn_fmed3f(t[j], -448.0f, 448.0f);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            int w = __builtin_amdgcn_cvt_pk_fp8_f32(t[4 * h], t[4 * h + 1], 0, false);
-            out[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t[4 * h + 2], t[4 * h + 3], w, true);
-        }
+        for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_fmed3f(v[j], -448.0f, 448.0f);
+        const int low = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], low, true);
     }
-    return out;
 }
 
-// The values 8 elements and their scale stand for: element times power of two, exact unless it overflows or is
+// The values 4 elements and their scale stand for: element times power of two, exact unless it overflows or is
 // below float32's least subnormal.
 template <int BITS>
-__device__ __forceinline__ void mx_decode(float (&v)[8], u32x2 codes, int scale) {
+__device__ __forceinline__ f32x4 mx_decode(uint32_t codes, int scale) {
     // 2^(scale - 127) as a float: subnormal for scale 0, NaN for 255
-    const float power = __uint_as_float(scale == 0 ? 0x00400000u : scale == kMxNan ? 0x7fc00000u : (uint32_t)scale << 23);
-    auto put = [&](int j, auto pair) { v[j] = pair[0], v[j + 1] = pair[1]; };
+    const float power = __uint_as_float(scale == 0        ? 0x00400000u
+                                        : scale == kMxNan ? 0x7fc00000u
+                                                          : (uint32_t)scale << 23);
+    f32x4 v;
+    auto put = [&](int j, auto pair) { v[j] = __fmul_rn(pair[0], power), v[j + 1] = __fmul_rn(pair[1], power); };
     if constexpr (BITS == 4) {
-        put(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 0));
-        put(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 1));
-        put(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 2));
-        put(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 3));
+        put(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 0));
+        put(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 1));
     } else {
-        put(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes[0], 1.0f, false));
-        put(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes[0], 1.0f, true));
-        put(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes[1], 1.0f, false));
-        put(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes[1], 1.0f, true));
+        put(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, 1.0f, false));
+        put(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, 1.0f, true));
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], power);
+    return v;
 }
 
 // Workgroups of a launch over two dimensions of the grid, so that none of them has 2^32 threads or more.

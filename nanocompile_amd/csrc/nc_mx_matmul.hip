@@ -217,15 +217,16 @@ __global__ __launch_bounds__(WAVES * 64) void mx_split(MxArgs a) {
     constexpr int kStep = 1024 * (NB * NF + MF * X::kCopies), kParts = WAVES * NB * MF * NF * 1024;
     __shared__ __align__(1024) uint8_t lds[WAVES * U * kStep > kParts ? WAVES * U * kStep : kParts];
 
-    const uint32_t mtiles = ((uint32_t)a.M + 16 * MF - 1) / (16 * MF), ntiles = ((uint32_t)a.N + 16 * NF - 1) / (16 * NF);
+    constexpr int BM = 16 * MF, BN = 16 * NF;
+    const uint32_t mtiles = ((uint32_t)a.M + BM - 1) / BM, ntiles = ((uint32_t)a.N + BN - 1) / BN;
     if (nc::workgroup_id() >= mtiles * ntiles) return;
     const Tile tile = tile_of((uint32_t)nc::workgroup_id(), mtiles, ntiles);
-    const int64_t m0 = tile.m * (16 * MF), n0 = tile.n * (16 * NF);
+    const int64_t m0 = tile.m * BM, n0 = tile.n * BN;
     const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), steps = a.steps;
     // The tile's first rows and a step's place in them are the same for every lane (scalar registers); a lane's
     // row and chunk are an offset of 32 bits.
-    const int x_last = (int)min(a.M - 1 - m0, (int64_t)16 * MF - 1), w_last = (int)min(a.N - 1 - n0, (int64_t)16 * NF - 1);
+    const int x_last = (int)min(a.M - 1 - m0, (int64_t)BM - 1), w_last = (int)min(a.N - 1 - n0, (int64_t)BN - 1);
     auto x_row = [&](int r) { return (uint32_t)(min(r, x_last) * steps); };
     auto w_row = [&](int r) { return (uint32_t)(min(r, w_last) * steps); };
     const uint8_t *xq = a.xq + (size_t)m0 * steps * (16 * BITS), *xs = a.xs + (size_t)m0 * steps * 4;
@@ -264,6 +265,7 @@ __global__ __launch_bounds__(WAVES * 64) void mx_split(MxArgs a) {
             for (int j = 0; j < NF; ++j) we[b][j] = load_words(ws[b] + (size_t)s * 4 + wsat[j]);
 #pragma unroll
         for (int i = 0; i < MF; ++i) xe[i] = load_words(xs + (size_t)s * 4 + xsat[i]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the steps before are read
 #pragma unroll
         for (int c = 0; c < C; ++c) {
 #pragma unroll
@@ -343,24 +345,25 @@ __global__ __launch_bounds__(WAVES * 64) void mx_split(MxArgs a) {
 template <int BITS, int NB, int MF, int NF, int WAVES, int U>
 int32_t launch_split(const MxArgs &a) {
     const int64_t tiles = (a.M + 16 * MF - 1) / (16 * MF) * ((a.N + 16 * NF - 1) / (16 * NF));
-    hipLaunchKernelGGL((mx_split<BITS, NB, MF, NF, WAVES, U>), nc::grid_of(tiles), dim3(WAVES * 64), 0, nc::stream(), a);
+    hipLaunchKernelGGL((mx_split<BITS, NB, MF, NF, WAVES, U>), nc::grid_of(tiles), dim3(WAVES * 64), 0, nc::stream(),
+                       a);
     return nc::launched("mx_split");
 }
 
-// copy_to_lds for copies that stay in flight past LDS reads: before any read of LDS the compiler waits for every copy it
-// knows of, as each might write what is read. Which copies a read needs is counted in mx_tile, so these are hidden
-// from it. They write no register; `to` goes through m0, which takes a wait state.
+// copy_to_lds for copies that stay in flight past LDS reads: before any read of LDS the compiler waits for every copy
+// it knows of, as each might write what is read. Which copies a read needs is counted in mx_tile, so these are
+// hidden from it. They write no register; `to` goes through m0, which takes a wait state.
 __device__ __forceinline__ void copy_to_lds_counted(const uint8_t *from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from),
                  "s"(__builtin_amdgcn_readfirstlane(to)) : "m0", "memory");
 }
 
 // Many outputs: a workgroup of WM x WN waves takes 32 MF WM rows of x by 32 NF WN weight rows (of each weight), each
-// wave 32 MF x 32 NF of them. Operands are staged in LDS two steps at a time: 4-bit rows are copied 128 bytes at a time,
-// as whole lines of the cache come twice as fast as halves (measured: 33 against 16 TB/s). A wave reads half a step's
-// operands into registers while it multiplies the half before.
-// With two buffers there is one barrier a pair of steps, before its last half: by then the next pair has landed and this
-// one is read, so the copies of the pair after next start, with two steps to land. With one the next pair's copies
+// wave 32 MF x 32 NF of them. Operands are staged in LDS two steps at a time: 4-bit rows are copied 128 bytes at a
+// time, as whole lines of the cache come twice as fast as halves (measured: 33 against 16 TB/s). A wave reads half a
+// step's operands into registers while it multiplies the half before.
+// With two buffers there is one barrier a pair of steps, before its last half: by then the next pair has landed and
+// this one is read, so the copies of the pair after next start, with two steps to land. With one the next pair's copies
 // start at that barrier and have landed at another, half a step later: other workgroups, of which a CU takes twice as
 // many, fill the wait. Where the steps are odd the last is the second of a pair whose first is not multiplied again.
 // The scales come four steps at a time, 16 bytes a row, with the pairs 0, 2, 4 ... The outputs go through LDS, a wave's
@@ -375,9 +378,9 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
     static_assert(WK == 1 || WM * WN == 1, "k is split over waves that have the whole tile each");
     using S = Stage<128, 2>;
     constexpr int WAVES = WM * WN, BM = 32 * MF * WM, BN = 32 * NF * WN, XH = BITS / 4;
-    constexpr int XC = BM / 8, WC = BN / 8, SC = (BM + NB * BN + 63) / 64;  // copies of 128-byte rows; of a group of scales
+    constexpr int XC = BM / 8, WC = BN / 8, SC = (BM + NB * BN + 63) / 64;      // copies of 128-byte rows, of scales
     constexpr int BUFFER = (XH * XC + NB * WC) * 1024;
-    constexpr int kScaleCopies = (SC + WAVES - 1) / WAVES, kCopies = (XH * XC + NB * WC) / WAVES;      // a wave's, of a pair
+    constexpr int kScaleCopies = (SC + WAVES - 1) / WAVES, kCopies = (XH * XC + NB * WC) / WAVES;   // a wave's
     constexpr int kOutRow = 32 * NF * 4 + 16;                       // bytes of LDS, and of it a wave has 32 rows
     static_assert(XC % WAVES == 0 && WC % WAVES == 0, "whole copies a wave");
     constexpr int kStaged = BUFFERS * (BUFFER + SC * 1024), kOut = WAVES * (WK == 1 ? 1 : NB) * 32 * kOutRow;
@@ -404,8 +407,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
         q[b] = a.q[b] + (size_t)n0 * steps * 64;
         ws[b] = a.ws[b] + (size_t)n0 * steps * 4;
     }
-    // This lane's part of the wave's copies: copies i * WAVES + wave of an operand, and of a group of scales. 8-bit rows
-    // are two 128-byte ones, a step each, the halves of a block four chunks apart.
+    // This lane's part of the wave's copies: copies i * WAVES + wave of an operand, and of a group of scales. 8-bit
+    // rows are two 128-byte ones, a step each, the halves of a block four chunks apart.
     uint32_t xat[XC / WAVES], wat[WC / WAVES];
     const uint8_t *sat[kScaleCopies];
 #pragma unroll
@@ -451,9 +454,10 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
     auto copy_scales = [&](int p) {
         const int first = min(p / 2 * 4, steps - 4);
 #pragma unroll
-        for (int i = 0; i < kScaleCopies; ++i)
-            copy_to_lds_counted(sat[i] + first * 4,
-                                base + BUFFERS * BUFFER + (p / 2 % BUFFERS * SC + min(i * WAVES + wave, SC - 1)) * 1024);
+        for (int i = 0; i < kScaleCopies; ++i) {
+            const int to = p / 2 % BUFFERS * SC + min(i * WAVES + wave, SC - 1);
+            copy_to_lds_counted(sat[i] + first * 4, base + BUFFERS * BUFFER + to * 1024);
+        }
     };
     // Half a step's operands: a lane's block g + 2 half of every row it multiplies.
     struct Half {
@@ -464,13 +468,13 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
         uint32_t x[MF], w[NB][NF];
     };
     constexpr int kReads = NB * NF + MF * XH, kRows = NB * NF + MF;        // LDS reads of a half, of a step's scales
-    // Read p of half `half` of step `step` (0, 1) of a buffer. (The second step's 4-bit blocks are chunks 4 .. 7 of a row.)
+    // Read p of half `half` of step `step` (0, 1) of a buffer. (The second step's 4-bit blocks are chunks 4 .. 7.)
     auto read_half = [&](Half &f, int buffer, int step, int half, int p) {
         const uint8_t *from = lds + buffer * BUFFER;
         const int block = g + 2 * half;
         if (p < NB * NF) {
-            f.w[p / NF][p % NF] = *reinterpret_cast<const i32x4 *>(from + (XH * XC + p / NF * WC) * 1024 + 32 * (p % NF) * 128 +
-                                                                   (S::at(wn + row, block, 0) ^ 64 * step));
+            f.w[p / NF][p % NF] = *reinterpret_cast<const i32x4 *>(
+                from + (XH * XC + p / NF * WC) * 1024 + 32 * (p % NF) * 128 + (S::at(wn + row, block, 0) ^ 64 * step));
         } else {
             const int i = (p - NB * NF) / XH, h = (p - NB * NF) % XH;
             f.x[i][h] = *reinterpret_cast<const i32x4 *>(
@@ -489,8 +493,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
         }
     };
     f32x16 acc[NB][MF][NF] = {};
-    // Half a step's products, the outputs acc[n = 8 (r / 4) + 4 (l / 32) + r % 4][m = l % 32]. `other(p)`, p < pieces, is
-    // the next half's reads and copies, spread between the products: in one place they would leave the matrix
+    // Half a step's products, the outputs acc[n = 8 (r / 4) + 4 (l / 32) + r % 4][m = l % 32]. `other(p)`, p < pieces,
+    // is the next half's reads and copies, spread between the products: in one place they would leave the matrix
     // core idle, as all waves come to them at once. 4 bits: 64 values of k in one instruction, which picks a scale's
     // byte itself.
     auto multiply = [&](const Half &f, const Scales &e, auto half, int pieces, auto other) {
@@ -531,7 +535,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
         }
     };
     // Half f, whose first part is in `part`; leaves the first part of half `half` of a step of scales e, f_next, there.
-    auto multiply_converted = [&](const Half &f, const Half &f_next, const Scales &e, int half, int pieces, auto other) {
+    auto multiply_converted = [&](const Half &f, const Half &f_next, const Scales &e, int half, int pieces,
+                                  auto other) {
         constexpr int products = NB * NF * MF;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -585,8 +590,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
             for (int i = 0; i < kRows; ++i) convert(part, f0, 0, i);
         }
     };
-    // A pair's second step (f0 and e1 hold its first half and scales); the next pair's first half read, of its second step
-    // where that is the last, odd one.
+    // A pair's second step (f0 and e1 hold its first half and scales); the next pair's first half read, of its second
+    // step where that is the last, odd one.
     auto second = [&](int p, auto which) {
         constexpr int B = decltype(which)::value;
         product(f0, f1, e1, e1, first_half, kReads, [&](int i) { read_half(f1, B, 1, 1, i); });
@@ -601,7 +606,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
             begin_pair(begin, 2 * p + 2);
         } else {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            meet();                                                 // pair p + 1 has landed, pair p is read, by every wave
+            meet();                                                 // pair p + 1 has landed and p is read, for all
             product(f1, f0, e1, e0, second_half, kReads + kRows + kCopies, [&](int i) {
                 if (i < kReads) read_half(f0, 1 - B, begin, 0, i);
                 else if (i < kReads + kRows) read_scales(e0, 2 * p + 2, i - kReads);
@@ -639,7 +644,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
                 first(p, std::integral_constant<int, 0>{});
                 second(p, std::integral_constant<int, 0>{});
             }
-            if (odd) {                                              // f0 and e0 hold the last step's first half and scales
+            if (odd) {                                              // f0, e0: the last step's first half and scales
                 product(f0, f1, e0, e0, first_half, kReads, [&](int i) { read_half(f1, 0, 1, 1, i); });
                 product(f1, f1, e0, e0, second_half, 0, [](int) {});
             }
@@ -663,9 +668,12 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
 #pragma unroll
             for (int j = 0; j < NF; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    *reinterpret_cast<f32x4 *>(lds + (b * 32 + row) * kOutRow + (32 * j + 8 * r + 4 * g) * 4) =
-                        f32x4{acc[b][0][j][4 * r], acc[b][0][j][4 * r + 1], acc[b][0][j][4 * r + 2], acc[b][0][j][4 * r + 3]};
+                for (int r = 0; r < 4; ++r) {
+                    f32x4 v;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[c] = acc[b][0][j][4 * r + c];
+                    *reinterpret_cast<f32x4 *>(lds + (b * 32 + row) * kOutRow + (32 * j + 8 * r + 4 * g) * 4) = v;
+                }
         __syncthreads();
         if (part_of_k * kMine >= kAll) return;
         const int down = part_of_k * (kMine * kDown) + lane / kAcross;
@@ -677,8 +685,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
             for (int w = 0; w < WK; ++w)
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
-                    sum[b] += *reinterpret_cast<const f32x4 *>(all_lds + w * kShare + (b * 32 + down + k * kDown) * kOutRow +
-                                                               lane % kAcross * 16);
+                    sum[b] += *reinterpret_cast<const f32x4 *>(
+                        all_lds + w * kShare + (b * 32 + down + k * kDown) * kOutRow + lane % kAcross * 16);
 #pragma unroll
             for (int c = 0; c < 4; ++c) v[k][c] = NB == 1 ? sum[0][c] : silu_times(sum[0][c], sum[NB - 1][c]);
         }
@@ -704,7 +712,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
         f32x4 v[32 / kDown];
 #pragma unroll
         for (int k = 0; k < 32 / kDown; ++k)
-            v[k] = *reinterpret_cast<const f32x4 *>(mine + (k * kDown + lane / kAcross) * kOutRow + lane % kAcross * 16);
+            v[k] =
+                *reinterpret_cast<const f32x4 *>(mine + (k * kDown + lane / kAcross) * kOutRow + lane % kAcross * 16);
         asm volatile("" ::: "memory");
         finish<NB, 32 / kDown>(a, m0 + wm + 32 * i + lane / kAcross, kDown, n, v);
     }

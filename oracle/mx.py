@@ -62,7 +62,8 @@ def dequantize(codes, scales, k: int):
 
 
 def norm(x, delta, gamma, eps: float):
-    """``(t, normed)`` float32: the sum of squares in 64 bits, its root's inverse rounded once, then float32 products."""
+    """``(t, normed)`` float32: the sum of squares in 64 bits, its root's inverse rounded once, then float32
+    products."""
     with np.errstate(all="ignore"):
         t = x if delta is None else (x + delta).astype(np.float32)
         t64 = t.astype(np.float64)
