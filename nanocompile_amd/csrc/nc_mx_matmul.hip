@@ -381,6 +381,9 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
     constexpr int XC = BM / 8, WC = BN / 8, SC = (BM + NB * BN + 63) / 64;      // copies of 128-byte rows, of scales
     constexpr int BUFFER = (XH * XC + NB * WC) * 1024;
     constexpr int kScaleCopies = (SC + WAVES - 1) / WAVES, kCopies = (XH * XC + NB * WC) / WAVES;   // a wave's
+    // Of a pair's copies into the second buffer, those that start a half later, with the pair before it: half in 8 bits
+    // (512 x 896 x 4864 10.6 us with none, 10.0 so; a pair of 1867 x 8192 x 8192 418 and 400), in 4 no quicker.
+    constexpr int kLate = BUFFERS == 2 && BITS == 8 ? kCopies / 2 : 0;
     constexpr int kOutRow = 32 * NF * 4 + 16;                       // bytes of LDS, and of it a wave has 32 rows
     static_assert(XC % WAVES == 0 && WC % WAVES == 0, "whole copies a wave");
     constexpr int kStaged = BUFFERS * (BUFFER + SC * 1024), kOut = WAVES * (WK == 1 ? 1 : NB) * 32 * kOutRow;
@@ -572,7 +575,10 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
     // A pair's first step (f0 and e0 hold its first half and scales), and then its second's first half read.
     auto first = [&](int p, auto which) {
         constexpr int B = decltype(which)::value;
-        product(f0, f1, e0, e0, first_half, kReads, [&](int i) { read_half(f1, B, 0, 1, i); });
+        product(f0, f1, e0, e0, first_half, kReads + kLate, [&](int i) {
+            if (i < kReads) read_half(f1, B, 0, 1, i);
+            else copy_piece(p + 1, 1 - B, kCopies - kLate + i - kReads);
+        });
         product(f1, f0, e0, e1, second_half, kReads + kRows, [&](int i) {
             if (i < kReads) read_half(f0, B, 1, 0, i);
             else read_scales(e1, first_step(p) + 1, i - kReads);
@@ -607,7 +613,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
         } else {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             meet();                                                 // pair p + 1 has landed and p is read, for all
-            product(f1, f0, e1, e0, second_half, kReads + kRows + kCopies, [&](int i) {
+            product(f1, f0, e1, e0, second_half, kReads + kRows + kCopies - kLate, [&](int i) {
                 if (i < kReads) read_half(f0, 1 - B, begin, 0, i);
                 else if (i < kReads + kRows) read_scales(e0, 2 * p + 2, i - kReads);
                 else copy_piece(p + 2, B, i - kReads - kRows);
@@ -627,10 +633,10 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
         if constexpr (BUFFERS == 2) {
             if (p_begin % 2 == 1) copy_scales(p_begin + 1);
 #pragma unroll
-            for (int i = 0; i < kCopies; ++i) copy_piece(p_begin + 1, 1, i);
+            for (int i = 0; i < kCopies - kLate; ++i) copy_piece(p_begin + 1, 1, i);
         }
         // (the second pair's scales may be waited for too)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BUFFERS == 2 ? kCopies : 0) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BUFFERS == 2 ? kCopies - kLate : 0) : "memory");
         meet();
         const int alone = odd && p_begin + 1 == p_end;              // nothing but the odd step
         begin_pair(alone, 2 * p_begin);
