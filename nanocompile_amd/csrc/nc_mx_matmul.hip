@@ -309,9 +309,6 @@ __global__ __launch_bounds__(WAVES * 64) void mx_split(MxArgs a) {
     const int share = (steps + WAVES - 1) / WAVES, end = min(steps, (wave + 1) * share);
     int s = wave * share;
     for (; s + U <= end; s += U) batch(s, std::integral_constant<int, U>{});
-    if constexpr (U > 2) {
-        if (s + 2 <= end) batch(s, std::integral_constant<int, 2>{}), s += 2;
-    }
     if constexpr (U > 1) {
         if (s < end) batch(s, std::integral_constant<int, 1>{});
     }
@@ -371,7 +368,7 @@ __device__ __forceinline__ void copy_to_lds_counted(const uint8_t *from, uint32_
 // took 255 us so, 140 of them without the stores).
 // With WK > 1 the tile is one wave's, and WK waves have the whole of it and a part of k each, with stages of their own
 // and so without barriers; their sums are added in the order of the waves. For the shapes whose tiles are few and k
-// long: 512 x 896 x 4864 in 4 bits 6.5 us (8.7 with 64 x 64 by four waves), 128 x 4096 x 4096 in 8 bits 8.7 (11.4 with
+// long: 512 x 896 x 4864 in 4 bits 6.5 us, in 8 bits 9.1; 128 x 4096 x 4096 in 8 bits 8.1 (8.7, 11.1 and 11.1 with
 // mx_split). Needs four steps.
 template <int BITS, int NB, int WM, int WN, int MF, int NF, int BUFFERS, int WK>
 __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {

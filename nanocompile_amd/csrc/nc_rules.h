@@ -191,19 +191,19 @@ constexpr int prefill_rows(int64_t M, int64_t heads, int64_t kv_heads, int64_t k
 //                     8/1: 13 x 4096 x 4096 4.8 / 4.0, 9 x 1305 x 4987 4.8 / 3.9; 8/2: 3 x 2048 x 8192 10.7 / 7.5
 //   kRow / kSplit     4/1: 76 x 1152 x 896 2.7 / 3.0, 199 x 918 x 287 2.9 / 2.8; 8/1: 250 x 896 x 896 3.9 / 3.6;
 //                     4/2: 58 x 4864 x 896 4.1 / 5.0; 8/2: 40 x 4864 x 896 4.5 / 5.8, 342 x 1439 x 1285 9.8 / 7.7
-//   kRow / kJoined    4/1: 105 x 896 x 4864 4.5 / 4.9, 146 x 896 x 4864 6.0 / 5.0; 8/1: 163 x 896 x 4864 7.7 / 9.2,
-//                     29 x 8192 x 8192 16.9 / 12.3; 4/2: 271 x 739 x 4251 12.1 / 7.1; 8/2: 53 x 3195 x 5597 15.1 / 11.1
+//   kRow / kJoined    4/1: 105 x 896 x 4864 4.5 / 4.9, 146 x 896 x 4864 6.0 / 5.0; 8/1: 163 x 896 x 4864 7.8 / 8.6,
+//                     29 x 8192 x 8192 16.6 / 12.5; 4/2: 271 x 739 x 4251 12.2 / 7.0; 8/2: 53 x 3195 x 5597 15.2 / 10.3
 //   kSplit / kJoined  4/1: 2021 x 161 x 1104 3.9 / 4.0, 134 x 4096 x 4096 11.5 / 8.0;
-//                     8/1: 455 x 2103 x 1397 8.4 / 10.2, 343 x 2048 x 8192 25.2 / 23.0
-//   kJoined / kDeep   8/2: 1076 x 693 x 3214 21.9 / 16.2; 4/2: 190 x 3139 x 2592 15.5 / 10.2
+//                     8/1: 455 x 2103 x 1397 8.4 / 10.0, 343 x 2048 x 8192 25.4 / 22.6
+//   kJoined / kDeep   8/2: 1076 x 693 x 3214 20.8 / 16.1; 4/2: 190 x 3139 x 2592 15.5 / 10.3
 //   kSmall / kDeep    4/1: 294 x 16000 x 1024 10.5 / 11.2, 2162 x 896 x 4864 17.4 / 14.8;
 //                     4/2: 99 x 4864 x 896 5.4 / 5.2
-//   kSmall / kMedium  4/1: 442 x 8192 x 8192 36.1 / 29.9; 8/1: 789 x 4096 x 4096 37.8 / 30.7
+//   kSmall / kMedium  4/1: 442 x 8192 x 8192 36.1 / 29.9; 8/1: 789 x 4096 x 4096 37.5 / 30.2
 //   kDeep / kMedium   4/1: 368 x 8192 x 2048 10.3 / 11.4, 923 x 8192 x 2048 20.9 / 16.6
 //   kMedium / kLarge  4/1: 923 x 8192 x 2048 16.6 / 20.7, 1960 x 8192 x 2048 30.2 / 26.0;
-//                     8/1: 1270 x 4988 x 4760 69.0 / 53.8
-//   kSmall / kLarge   4/2: 465 x 4864 x 896 8.6 / 13.9, 3887 x 4096 x 4096 110 / 71; 8/2: 993 x 4864 x 896 21.6 / 28.7,
-//                     1867 x 8192 x 8192 432 / 372
+//                     8/1: 1270 x 4988 x 4760 68.4 / 53.1
+//   kSmall / kLarge   4/2: 465 x 4864 x 896 8.6 / 13.9, 3887 x 4096 x 4096 103 / 71; 8/2: 993 x 4864 x 896 21.9 / 27.4,
+//                     1867 x 8192 x 8192 426 / 369
 enum class MxTile { kRow, kLongRow, kSplit, kJoined, kSmall, kDeep, kMedium, kLarge };
 
 constexpr MxTile mx_tile(int64_t M, int64_t N, int64_t steps, int bits, int weights) {

@@ -334,6 +334,117 @@ def test_residual_in_place_and_guards(gpu, m, n, k):
     assert (got[:4] == 0xA5).all() and (got[-4:] == 0xA5).all()
 
 
+# one shape for each kernel of many outputs or long k (4 and 8 bits alike): k split over waves, 64 x 64 by two steps and
+# by four, the larger ones
+KINDS = [(330, 1001, 1537), (1281, 1025, 513), (1281, 1025, 1100), (1793, 1921, 1537), (3203, 3201, 1030)]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("m,n,k", KINDS)
+def test_every_kind_in_place_with_bad_blocks(gpu, m, n, k, bits):
+    """y over the residual between guards, twice the same bits; NaN blocks in the first and the last step spoil their
+    row or column and no other output."""
+    from nanocompile_amd import hip, kernels
+    from nanocompile_amd.hip import DeviceArray
+    rng = np.random.default_rng(k)
+    (xq, xs), (w, u) = operands(rng, m, n, k, bits, 2)
+    residual = rng.standard_normal((m, n)).astype(np.float32)
+    bias = rng.standard_normal(n).astype(np.float32)
+    dx, dq, du, duq = (DeviceArray.from_host(a) for a in (xq, w[0], u[1], u[0]))
+    db, r = DeviceArray.from_host(bias), DeviceArray.from_host(residual)
+    clean = kernels.matmul_mx(dx, xs, dq, w[1], db, r).numpy()
+    pair = kernels.matmul_mx_swiglu(dx, xs, dq, w[1], duq, du).numpy()
+    xs2, ws2 = xs.copy(), w[1].copy()
+    xs2[m - 1, (k - 1) // 32] = ws2[n - 1, 0] = xs2[m // 2, 0] = ws2[n // 3, (k - 1) // 32] = 255
+    bad = np.zeros((m, n), bool)
+    bad[[m // 2, m - 1]], bad[:, [n // 3, n - 1]] = True, True
+    for scales in ((xs, w[1]), (xs, w[1]), (xs2, ws2)):
+        held = [DeviceArray.from_host(a) for a in scales]
+        p, read = guarded(residual.nbytes + 8)
+        y = DeviceArray((m, n), np.float32, ptr=p + 4, owner=False)
+        y.upload(residual)
+        hip.call("nc_matmul_mx", [y, dx, held[0], dq, held[1], db, y], [m, n, k, bits])
+        hip.sync()
+        whole = read()
+        assert (whole[:4] == 0xA5).all() and (whole[-4:] == 0xA5).all()
+        got = whole[4:-4].view(np.float32).reshape(m, n)
+        h = kernels.matmul_mx_swiglu(dx, held[0], dq, held[1], duq, du).numpy()
+        for out, want in ((got, clean), (h, pair)):
+            if scales[0] is xs:
+                assert np.array_equal(float_bits_of(out), float_bits_of(want))
+            else:
+                assert np.isnan(out[bad]).all()
+                assert np.array_equal(float_bits_of(out[~bad]), float_bits_of(want[~bad]))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("m,n,k", KINDS)
+def test_every_position_of_k_counts_once_in_every_kind(gpu, m, n, k, bits):
+    """One nonzero product a row, row i's at k = i mod K and then at others till every k was: exact."""
+    from nanocompile_amd import kernels
+    w = np.exp2(np.arange(k) % 4 + np.arange(k) // 32 % 5)[None, :] * (1 + np.arange(n) % 2)[:, None]
+    wq = mx.quantize(w.astype(np.float32), 4)
+    assert np.array_equal(mx.dequantize(*wq, k), w)
+    for first in range(0, k, m):
+        at = (first + np.arange(m)) % k
+        x = np.zeros((m, k), np.float32)
+        x[np.arange(m), at] = np.exp2(at // 32 - 8)
+        got = kernels.matmul_mx(*mx.quantize(x, bits), *wq).numpy()
+        assert np.array_equal(got, np.exp2(at // 32 - 8)[:, None] * w.T[at]), first
+
+
+# -- more workgroups than one row of the grid ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_long_arrays_of_rows(gpu, bits):
+    """140,003 rows of 1,000: the rows about the grid's first border and the last against the definition."""
+    from nanocompile_amd import kernels
+    from nanocompile_amd.hip import DeviceArray
+    m, k = 140003, 1000
+    rng = np.random.default_rng(bits)
+    x = rng.standard_normal((m, k), dtype=np.float32)
+    q, scales = kernels.quantize_mx(DeviceArray.from_host(x), bits)
+    back = kernels.dequantize_mx(q, scales, k).numpy()
+    q, scales = q.numpy(), scales.numpy()
+    per_row = 1024
+    for values in (8, 4):                              # a thread's, in one kernel and the other
+        border = 65536 * 256 * values // per_row
+        for rows in (slice(0, 3), slice(border - 2, border + 3), slice(m - 3, m)):
+            want = mx.quantize(x[rows], bits)
+            assert np.array_equal(q[rows], want[0]) and np.array_equal(scales[rows], want[1])
+            assert same_bits(back[rows], mx.dequantize(*want, k))
+
+
+@pytest.mark.parametrize("mx_bits", [0, 8])
+def test_norm_of_many_rows(gpu, mx_bits):
+    from nanocompile_amd import kernels
+    m, k = 4 * 65536 + 70, 5
+    rng = np.random.default_rng(mx_bits)
+    x, gamma = rng.standard_normal((m, k)).astype(np.float32), np.ones(k, np.float32)
+    t, _, q, qs = kernels.add_rms_norm_quant(x, None, gamma, 1e-6, mx_bits=mx_bits)
+    _, n = mx.norm(x, None, gamma, 1e-6)
+    want = mx.quantize(n, 8) if mx_bits else R.quantize_token(n)
+    assert np.array_equal(q.numpy(), want[0]) and same_bits(qs.numpy(), want[1])
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 1200017, 40), (16500, 16400, 600)])
+def test_products_of_many_tiles(gpu, m, n, k):
+    """75,002 tiles of 16 x 16, 66,306 of 64 x 64: whole rows about the borders against the definition."""
+    from nanocompile_amd import kernels
+    x, (w,) = operands(np.random.default_rng(m), m, n, k, 4)
+    y = kernels.matmul_mx(*x, *w).numpy()
+    for rows in ([0, m - 1], [m // 2]):
+        for columns in (slice(0, 300), slice(n // 2, n // 2 + 300), slice(n - 300, n)):
+            want, size = mx.matmul(x[0][rows], x[1][rows], w[0][columns], w[1][columns])
+            assert (np.abs(y[rows, columns] - want) <= product_error(size, k, 4)).all()
+    assert np.isfinite(y).all()
+    x[1][:] = w[1][:] = 127                            # every scale 1, all elements: no output is left unwritten
+    x[0][:] = w[0][:] = 0x22                           # ones
+    ones = kernels.matmul_mx(*x, *w).numpy()
+    assert (ones == x[0].shape[1] * 2).all()
+
+
 # -- together ------------------------------------------------------------------------------------------
 
 

@@ -34,6 +34,13 @@ def test_the_products_tests_reach_every_kind(run, bits, weights):  # noqa: F811
     assert reached == set(range(8)) - ({MEDIUM} if weights == 2 else set())
 
 
+@pytest.mark.parametrize("weights", [1, 2])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_one_shape_of_each_kind(run, bits, weights):  # noqa: F811
+    reached = set(kinds(run, [(bits, weights, *shape) for shape in test_mx_gpu.KINDS]))
+    assert reached == {JOINED, SMALL, DEEP, LARGE} | ({MEDIUM} if weights == 1 else set())
+
+
 def test_what_the_kernels_need(run):  # noqa: F811
     """Four steps for the kernels of whole tiles, twelve for the one that splits them; never the pair's missing kind;
     the largest shapes without overflow."""
