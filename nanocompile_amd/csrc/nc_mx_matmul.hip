@@ -750,7 +750,10 @@ int32_t launch(const MxArgs &a) {
             return launch_tile<BITS, NB, 1, 1, 1, BITS == 8 && NB == 1 ? 2 : 1, BITS == 4 && NB == 1 ? 1 : 2, 4>(a);
         case nc::MxTile::kDeep: return launch_tile<BITS, NB, 2, 2, 1, 1, 2>(a);
         case nc::MxTile::kMedium:
-            if constexpr (NB == 1) return launch_tile<BITS, NB, 2, 2, BITS == 4 ? 2 : 1, 2, 2>(a);
+            if constexpr (BITS == 8) return launch_tile<8, NB, 2, 2, NB, 3 - NB, 1>(a);
+            [[fallthrough]];                                        // (4 bits do not have it)
+        case nc::MxTile::kMediumDeep:
+            if constexpr (NB == 1) return launch_tile<BITS, 1, 2, 2, BITS == 4 ? 2 : 1, 2, 2>(a);
             [[fallthrough]];                                        // (no pair has it)
         case nc::MxTile::kSmall: return launch_tile<BITS, NB, 2, 2, 1, 1, 1>(a);
         case nc::MxTile::kLarge: return launch_tile<BITS, NB, 2, 4, BITS == 4 ? 4 : 2, NB == 1 ? 2 : 1, 2>(a);

@@ -184,7 +184,8 @@ constexpr int prefill_rows(int64_t M, int64_t heads, int64_t kv_heads, int64_t k
 //   kSplit          32 x 32, k over 4 waves of that kind; the only one for fewer than four steps and many outputs
 //   kJoined         32 x 32 (x 64 for 8 bits by one weight), k over 4 waves with the larger tiles' pipeline
 //   kSmall, kDeep   64 x 64 over 4 waves, two steps' operands in LDS or four
-//   kMedium         128 x 128 (64 x 128 for 8 bits), of one weight
+//   kMedium         64 x 128, two steps' operands; 128 x 64 for a pair; 8 bits only
+//   kMediumDeep     64 x 128, four steps' (128 x 128 for 4 bits); of one weight
 //   kLarge          256 x 256 (128 x 256 for 8 bits), half as wide for a pair
 // Both sides of each border, us (bits/weights: M x N x K):
 //   kRow / kLongRow   4/1: 2 x 4864 x 896 2.6 / 3.0, 2 x 8192 x 8192 7.3 / 7.8, 3 x 726 x 6801 4.2 / 3.9;
@@ -198,13 +199,16 @@ constexpr int prefill_rows(int64_t M, int64_t heads, int64_t kv_heads, int64_t k
 //   kJoined / kDeep   8/2: 1076 x 693 x 3214 20.8 / 16.1; 4/2: 190 x 3139 x 2592 15.5 / 10.3
 //   kSmall / kDeep    4/1: 294 x 16000 x 1024 10.5 / 11.2, 2162 x 896 x 4864 17.4 / 14.8;
 //                     4/2: 99 x 4864 x 896 5.4 / 5.2
-//   kSmall / kMedium  4/1: 442 x 8192 x 8192 36.1 / 29.9; 8/1: 789 x 4096 x 4096 37.5 / 30.2
-//   kDeep / kMedium   4/1: 368 x 8192 x 2048 10.3 / 11.4, 923 x 8192 x 2048 20.9 / 16.6
-//   kMedium / kLarge  4/1: 923 x 8192 x 2048 16.6 / 20.7, 1960 x 8192 x 2048 30.2 / 26.0;
-//                     8/1: 1270 x 4988 x 4760 68.4 / 53.1
-//   kSmall / kLarge   4/2: 465 x 4864 x 896 8.6 / 13.9, 3887 x 4096 x 4096 103 / 71; 8/2: 993 x 4864 x 896 21.9 / 27.4,
-//                     1867 x 8192 x 8192 426 / 369
-enum class MxTile { kRow, kLongRow, kSplit, kJoined, kSmall, kDeep, kMedium, kLarge };
+//   kSmall / kMedium  8/1: 900 x 2557 x 808 10.3 / 11.6, 2000 x 4864 x 896 26.4 / 24.1;
+//                     8/2: 400 x 4864 x 896 13.7 / 15.2, 2048 x 4864 x 896 39.9 / 37.1
+//   kDeep / kMediumDeep  4/1: 368 x 8192 x 2048 10.3 / 11.4, 923 x 8192 x 2048 20.9 / 16.6;
+//                     8/1: 700 x 896 x 4864 17.7 / 21.2, 320 x 4096 x 4096 20.7 / 18.4
+//   kMedium / kMediumDeep  8/1: 700 x 4096 x 4096 32.5 / 30.4, 1100 x 8192 x 2048 41.9 / 43.5
+//   kMediumDeep / kLarge  4/1: 923 x 8192 x 2048 16.6 / 20.7, 1960 x 8192 x 2048 30.2 / 26.0
+//   kMedium / kLarge  8/1: 1500 x 4096 x 4096 49.6 / 46.8, 4000 x 4864 x 896 42.2 / 47.4; 8/2: 640 x 4864 x 896
+//                     16.6 / 15.4, 4000 x 4864 x 2048 129 / 134, 1867 x 8192 x 8192 405 / 369
+//   kSmall / kLarge   4/2: 465 x 4864 x 896 8.6 / 13.9, 3887 x 4096 x 4096 103 / 71
+enum class MxTile { kRow, kLongRow, kSplit, kJoined, kSmall, kDeep, kMedium, kMediumDeep, kLarge };
 
 constexpr MxTile mx_tile(int64_t M, int64_t N, int64_t steps, int bits, int weights) {
     auto tiles = [&](int64_t rows, int64_t columns) { return (M + rows - 1) / rows * ((N + columns - 1) / columns); };
@@ -214,11 +218,14 @@ constexpr MxTile mx_tile(int64_t M, int64_t N, int64_t steps, int bits, int weig
     if (steps < 4) return MxTile::kSplit;
     if (work < 300) return steps >= 12 ? MxTile::kJoined : MxTile::kSplit;
     // kLarge has one workgroup on each of the 256 CUs: where its last round of them would be mostly empty, or the rows
-    // past M and N much of its work, smaller ones are quicker
-    const int64_t rows = bits == 4 ? 256 : 128, columns = 256 / weights;
-    const int64_t places = (tiles(rows, columns) + 255) / 256 * 256 * rows * columns;
-    if (steps >= 8 && M * N >= places / 5 * 3) return MxTile::kLarge;
-    if (weights == 1 && work >= 800 && steps >= 12) return MxTile::kMedium;
+    // past M and N much of its work, smaller ones are quicker; of several rounds each waits for its first copies and
+    // its stores, which takes long k to be worth it
+    const int64_t rows = bits == 4 ? 256 : 128, columns = 256 / weights, rounds = (tiles(rows, columns) + 255) / 256;
+    const bool full = M * N >= rounds * 256 * rows * columns / 5 * 3;
+    const int64_t enough = bits == 4 ? 8 : weights == 1 ? 12 : 32;
+    if (full && (steps >= enough || (bits == 8 && rounds == 1))) return MxTile::kLarge;
+    if (weights == 1 && steps >= 12 && (bits == 4 ? work >= 800 : work < 1100)) return MxTile::kMediumDeep;
+    if (bits == 8 && work >= 800 * weights) return MxTile::kMedium;
     return steps >= 8 && work < 800 ? MxTile::kDeep : MxTile::kSmall;
 }
 

@@ -258,7 +258,8 @@ SHORT = [(330, 1001, 1100), (701, 700, 300), (355, 1003, 600)]
 
 # many outputs again: 64 x 64 tiles of eight steps and more, the larger ones, their borders ragged
 TILES = [(1300, 1000, 1024), (1281, 1025, 1100), (1300, 1030, 1153), (1281, 1000, 513), (1800, 1900, 1537), (1793, 1921, 2560),
-         (3200, 3201, 1100), (3203, 3200, 1024), (3210, 3210, 1300)]
+         (3200, 3201, 1100), (3203, 3200, 1024), (3210, 3210, 1300), (3210, 3215, 1537), (2300, 2403, 1100),
+         (1650, 1701, 900), (2301, 2400, 4100)]
 
 
 @pytest.mark.parametrize("bits", [4, 8])
@@ -334,9 +335,10 @@ def test_residual_in_place_and_guards(gpu, m, n, k):
     assert (got[:4] == 0xA5).all() and (got[-4:] == 0xA5).all()
 
 
-# one shape for each kernel of many outputs or long k (4 and 8 bits alike): k split over waves, 64 x 64 by two steps and
-# by four, the larger ones
-KINDS = [(330, 1001, 1537), (1281, 1025, 513), (1281, 1025, 1100), (1793, 1921, 1537), (3203, 3201, 1030)]
+# a shape for each kernel of many outputs or long k: k split over waves, 64 x 64 by two steps and by four, the larger
+# ones
+KINDS = [(330, 1001, 1537), (1281, 1025, 513), (1281, 1025, 1100), (1793, 1921, 1537), (2301, 2403, 1030),
+         (3203, 3201, 1030)]
 
 
 @pytest.mark.parametrize("bits", [4, 8])
