@@ -41,6 +41,10 @@ struct MxArgs {
 
 // The scale's power of two, 255 as NaN: the conversions and matrix instructions read the exponent only.
 __device__ __forceinline__ float power(int scale) { return __int_as_float(scale << 23); }
+// That of byte `at` / 8 of four: the conversions ignore the bits about it (checked for every scale and element).
+__device__ __forceinline__ float power_at(uint32_t scales, int at) {
+    return __uint_as_float(__builtin_amdgcn_alignbit(scales, scales, at + 9));
+}
 
 // A lane's block of 32 values of a step, ready to multiply: 4-bit codes and their scale, or bfloat16 values.
 template <int BITS>
@@ -527,13 +531,13 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void mx_tile(MxArgs a) {
         float x[MF], w[NB][NF];
     } powers;
     auto take_powers = [&](const Scales &e, int half) {
-        const int shift = 8 * g + 16 * half;
+        const int at = 8 * g + 16 * half;
 #pragma unroll
-        for (int i = 0; i < MF; ++i) powers.x[i] = power(e.x[i] >> shift & 255);
+        for (int i = 0; i < MF; ++i) powers.x[i] = power_at(e.x[i], at);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int j = 0; j < NF; ++j) powers.w[b][j] = power(e.w[b][j] >> shift & 255);
+            for (int j = 0; j < NF; ++j) powers.w[b][j] = power_at(e.w[b][j], at);
     };
     auto convert = [&](Part &to, const Half &f, int t, int p) {
         if (p < NB * NF) {

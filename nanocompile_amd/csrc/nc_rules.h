@@ -206,7 +206,7 @@ constexpr int prefill_rows(int64_t M, int64_t heads, int64_t kv_heads, int64_t k
 //   kMedium / kMediumDeep  8/1: 700 x 4096 x 4096 32.5 / 30.4, 1100 x 8192 x 2048 41.9 / 43.5
 //   kMediumDeep / kLarge  4/1: 923 x 8192 x 2048 16.6 / 20.7, 1960 x 8192 x 2048 30.2 / 26.0
 //   kMedium / kLarge  8/1: 1500 x 4096 x 4096 49.6 / 46.8, 4000 x 4864 x 896 42.2 / 47.4; 8/2: 640 x 4864 x 896
-//                     16.6 / 15.4, 4000 x 4864 x 2048 129 / 134, 1867 x 8192 x 8192 405 / 369
+//                     16.6 / 15.4, 4000 x 4864 x 2048 129 / 134, 1867 x 8192 x 8192 375 / 385
 //   kSmall / kLarge   4/2: 465 x 4864 x 896 8.6 / 13.9, 3887 x 4096 x 4096 103 / 71
 enum class MxTile { kRow, kLongRow, kSplit, kJoined, kSmall, kDeep, kMedium, kMediumDeep, kLarge };
 
@@ -219,11 +219,11 @@ constexpr MxTile mx_tile(int64_t M, int64_t N, int64_t steps, int bits, int weig
     if (work < 300) return steps >= 12 ? MxTile::kJoined : MxTile::kSplit;
     // kLarge has one workgroup on each of the 256 CUs: where its last round of them would be mostly empty, or the rows
     // past M and N much of its work, smaller ones are quicker; of several rounds each waits for its first copies and
-    // its stores, which takes long k to be worth it
+    // its stores, which takes long k to be worth it (and never is for a pair in 8 bits)
     const int64_t rows = bits == 4 ? 256 : 128, columns = 256 / weights, rounds = (tiles(rows, columns) + 255) / 256;
     const bool full = M * N >= rounds * 256 * rows * columns / 5 * 3;
-    const int64_t enough = bits == 4 ? 8 : weights == 1 ? 12 : 32;
-    if (full && (steps >= enough || (bits == 8 && rounds == 1))) return MxTile::kLarge;
+    const bool several = bits == 4 ? steps >= 8 : weights == 1 && steps >= 12;
+    if (full && (several || (bits == 8 && rounds == 1))) return MxTile::kLarge;
     if (weights == 1 && steps >= 12 && (bits == 4 ? work >= 800 : work < 1100)) return MxTile::kMediumDeep;
     if (bits == 8 && work >= 800 * weights) return MxTile::kMedium;
     return steps >= 8 && work < 800 ? MxTile::kDeep : MxTile::kSmall;

@@ -22,7 +22,7 @@ def test_where_each_measured_quicker(run):  # noqa: F811
              (4, 1, 76, 1152, 896, ROW), (4, 1, 199, 918, 287, SPLIT), (4, 1, 2021, 161, 1104, SPLIT),
              (4, 1, 146, 896, 4864, JOINED), (8, 2, 53, 3195, 5597, JOINED), (4, 2, 190, 3139, 2592, DEEP),
              (4, 1, 2162, 896, 4864, DEEP), (4, 2, 465, 4864, 896, SMALL), (4, 1, 923, 8192, 2048, MEDIUM_DEEP),
-             (8, 1, 789, 4096, 4096, MEDIUM_DEEP), (4, 1, 1960, 8192, 2048, LARGE), (8, 2, 1867, 8192, 8192, LARGE),
+             (8, 1, 789, 4096, 4096, MEDIUM_DEEP), (4, 1, 1960, 8192, 2048, LARGE), (8, 2, 1867, 8192, 8192, MEDIUM),
              (8, 2, 48, 32000, 2048, SMALL), (8, 1, 2000, 4864, 896, MEDIUM), (8, 2, 1000, 4864, 896, MEDIUM),
              (8, 2, 640, 4864, 896, LARGE), (4, 1, 1, 151936, 896, ROW), (4, 1, 1, 1, 1, ROW)]
     assert kinds(run, [c[:-1] for c in cases]) == [c[-1] for c in cases]
