@@ -114,17 +114,16 @@ __device__ __forceinline__ f32x4 mx_step(const Block<8> &w, const Block<8> &x, f
 
 __device__ __forceinline__ void pin(f32x4 &v) { asm volatile("" : "+v"(v)); }
 
-// silu(g) * u = g * sigmoid(g) * u with e = exp(-|g|): sigmoid = (g < 0 ? e : 1) / (1 + e). nc::silu_mul takes the
-// exponential in double, to the reference's bits; here float32 is enough, and 5 million outputs took 10 us of it.
-// exp2's argument t keeps what its product with log2(e) rounds off, so e is good to two units in the last place,
-// the result to five; e under 2^-126 counts as 0.
+// silu(g) * u = g / (1 + exp(-g)) * u. nc::silu_mul takes the exponential in double, to the reference's bits; here
+// float32 is enough, and 5 million outputs took 10 us of it. exp2's argument t keeps what its product with log2(e)
+// rounds off, so the exponential is good to three units in the last place, the result to six; a sigmoid under 2^-126
+// counts as 0.
 __device__ __forceinline__ float silu_times(float g, float u) {
-    const float a = fminf(fabsf(g), 150.0f);           // (past 104 e is 0; an infinite g has sigmoid 0 or 1)
+    const float a = __builtin_amdgcn_fmed3f(g, -150.0f, 150.0f);       // (past 104 either way it is 0 or 1)
     const float t = __fmul_rn(a, -1.44269502f);        // log2(e) = 1.44269502 + 1.9259e-8
-    const float low = fmaf(a, -1.44269502f, -t) - a * 1.92596299e-8f;
-    const float e0 = __builtin_amdgcn_exp2f(t), e = fmaf(e0, low * 0.693147182f, e0);
-    const float sigmoid = (g < 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
-    return g * sigmoid * u;
+    const float low = fmaf(a, -1.92596299e-8f, fmaf(a, -1.44269502f, -t));
+    const float e = __fmul_rn(__builtin_amdgcn_exp2f(t), fmaf(low, 0.693147182f, 1.0f));
+    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
 // Outputs n .. n + 3 of rows m, m + apart, .. (R of them) from their sums, of a pair's from its products: + bias, the

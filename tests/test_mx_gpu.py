@@ -240,6 +240,30 @@ def check_swiglu(m, n, k, bits, seed=0):
     assert (np.abs(got - want) <= most).all()
 
 
+@pytest.mark.parametrize("m", [1, 1290])
+def test_silu_over_its_range(gpu, m):
+    """Gates that are one weight each, of either sign from 2^-127 to 6 * 2^100, exact; up 1: silu within 8 steps of
+    float32, or of the gate times 2^-126 where the sigmoid is less than that."""
+    from nanocompile_amd import kernels
+    scales = np.arange(0, 228, dtype=np.uint8)
+    n, k = 16 * len(scales), 520                       # 16 elements under every scale
+    gate = np.zeros((n, 5 * 64), np.uint8), np.full((n, 5 * 4), 127, np.uint8)
+    gate[0][:, 0], gate[1][:, 0] = np.arange(n) % 16, np.repeat(scales, 16)
+    up = np.zeros_like(gate[0]), np.full_like(gate[1], 127)
+    up[0][:, 0] = 2                                    # 1
+    x = np.zeros((m, 5 * 128), np.uint8), np.full((m, 5 * 4), 127, np.uint8)
+    x[0][:, 0] = 0x38                                  # 1
+    g = mx.dequantize(*gate, k)[:, 0].astype(np.float64)
+    with np.errstate(over="ignore"):
+        want = g / (1 + np.exp(-g))
+    got = kernels.matmul_mx_swiglu(*x, *gate, *up).numpy()
+    assert (np.abs(got - want) <= 16 * HALF * np.abs(want) + 2.0 ** -126 * np.abs(g) + 2.0 ** -149).all()
+    x4 = np.zeros((m, 5 * 64), np.uint8)
+    x4[:, 0] = 2
+    got = kernels.matmul_mx_swiglu(x4, x[1], *gate, *up).numpy()
+    assert (np.abs(got - want) <= 16 * HALF * np.abs(want) + 2.0 ** -126 * np.abs(g) + 2.0 ** -149).all()
+
+
 SHAPES = [(1, 1, 1), (1, 17, 32), (2, 16, 129), (3, 203, 100), (15, 64, 896), (16, 16, 128), (17, 33, 257), (31, 1, 640),
           (33, 130, 1040), (64, 96, 384), (65, 257, 1000), (130, 131, 512), (300, 65, 130), (1, 896, 4864), (5, 1152, 896),
           (129, 128, 4864), (257, 384, 896)]
