@@ -748,6 +748,9 @@ int32_t launch(const MxArgs &a) {
     switch (nc::mx_tile(a.M, a.N, a.steps, BITS, NB)) {
         case nc::MxTile::kRow: return launch_split<BITS, NB, 1, 1, 4, 2>(a);
         case nc::MxTile::kLongRow: return launch_split<BITS, NB, 1, 1, 8, 2>(a);
+        case nc::MxTile::kWideRow:
+            if constexpr (BITS == 8 && NB == 1) return launch_split<8, 1, 1, 2, 8, 2>(a);
+            [[fallthrough]];                                        // (no other has it)
         case nc::MxTile::kSplit: return launch_split<BITS, NB, 2, 2, 4, NB == 1 ? 2 : 1>(a);
         case nc::MxTile::kJoined:
             return launch_tile<BITS, NB, 1, 1, 1, BITS == 8 && NB == 1 ? 2 : 1, BITS == 4 && NB == 1 ? 1 : 2, 4>(a);

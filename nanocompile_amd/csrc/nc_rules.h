@@ -181,6 +181,7 @@ constexpr int prefill_rows(int64_t M, int64_t heads, int64_t kv_heads, int64_t k
 // workgroup's tile, as the operands are then read less often; the fewer, the more waves share one tile's k, as the
 // chip would stay empty:
 //   kRow, kLongRow  16 x 16 outputs, k over 4 or 8 waves that each copy their rows by themselves
+//   kWideRow        16 x 32, k over 8; 8 bits by one weight, whose copies are twice the row's and so fewer in flight
 //   kSplit          32 x 32, k over 4 waves of that kind; the only one for fewer than four steps and many outputs
 //   kJoined         32 x 32 (x 64 for 8 bits by one weight), k over 4 waves with the larger tiles' pipeline
 //   kSmall, kDeep   64 x 64 over 4 waves, two steps' operands in LDS or four
@@ -190,6 +191,9 @@ constexpr int prefill_rows(int64_t M, int64_t heads, int64_t kv_heads, int64_t k
 // Both sides of each border, us (bits/weights: M x N x K):
 //   kRow / kLongRow   4/1: 2 x 4864 x 896 2.6 / 3.0, 2 x 8192 x 8192 7.3 / 7.8, 3 x 726 x 6801 4.2 / 3.9;
 //                     8/1: 13 x 4096 x 4096 4.8 / 4.0, 9 x 1305 x 4987 4.8 / 3.9; 8/2: 3 x 2048 x 8192 10.7 / 7.5
+//   kRow / kWideRow   8/1: 8 x 8192 x 8192 9.6 / 8.4, 12 x 8192 x 2048 3.9 / 3.6, 8 x 28672 x 4096 14.8 / 13.4,
+//                     163 x 896 x 4864 7.8 / 8.6; 4/1: 8 x 8192 x 8192 7.8 / 7.6, 4 x 16000 x 1024 3.3 / 3.8
+//   kLongRow / kWideRow  8/1: 13 x 4096 x 4096 4.0 / 4.9, 73 x 1159 x 2905 4.6 / 4.2
 //   kRow / kSplit     4/1: 76 x 1152 x 896 2.7 / 3.0, 199 x 918 x 287 2.9 / 2.8; 8/1: 250 x 896 x 896 3.9 / 3.6;
 //                     4/2: 58 x 4864 x 896 4.1 / 5.0; 8/2: 40 x 4864 x 896 4.5 / 5.8, 342 x 1439 x 1285 9.8 / 7.7
 //   kRow / kJoined    4/1: 105 x 896 x 4864 4.5 / 4.9, 146 x 896 x 4864 6.0 / 5.0; 8/1: 163 x 896 x 4864 7.8 / 8.6,
@@ -208,13 +212,17 @@ constexpr int prefill_rows(int64_t M, int64_t heads, int64_t kv_heads, int64_t k
 //   kMedium / kLarge  8/1: 1500 x 4096 x 4096 49.6 / 46.8, 4000 x 4864 x 896 42.2 / 47.4; 8/2: 640 x 4864 x 896
 //                     16.6 / 15.4, 4000 x 4864 x 2048 129 / 134, 1867 x 8192 x 8192 375 / 385
 //   kSmall / kLarge   4/2: 465 x 4864 x 896 8.6 / 13.9, 3887 x 4096 x 4096 103 / 71
-enum class MxTile { kRow, kLongRow, kSplit, kJoined, kSmall, kDeep, kMedium, kMediumDeep, kLarge };
+enum class MxTile { kRow, kLongRow, kWideRow, kSplit, kJoined, kSmall, kDeep, kMedium, kMediumDeep, kLarge };
 
 constexpr MxTile mx_tile(int64_t M, int64_t N, int64_t steps, int bits, int weights) {
     auto tiles = [&](int64_t rows, int64_t columns) { return (M + rows - 1) / rows * ((N + columns - 1) / columns); };
     const int64_t t32 = tiles(32, 32), work = tiles(64, 64) * weights;
     const bool few = steps < 20 ? t32 < 170 * weights : tiles(32, bits == 8 && weights == 1 ? 64 : 32) < 110;
-    if (M <= 16 || few) return steps >= 10 && t32 <= 130 ? MxTile::kLongRow : MxTile::kRow;
+    if (M <= 16 || few) {
+        const int64_t wide = tiles(16, 32);
+        if (bits == 8 && weights == 1 && steps >= 12 && wide > 140 && (M <= 16 || wide <= 300)) return MxTile::kWideRow;
+        return steps >= 10 && t32 <= 130 ? MxTile::kLongRow : MxTile::kRow;
+    }
     if (steps < 4) return MxTile::kSplit;
     if (work < 300) return steps >= 12 ? MxTile::kJoined : MxTile::kSplit;
     // kLarge has one workgroup on each of the 256 CUs: where its last round of them would be mostly empty, or the rows

@@ -266,7 +266,7 @@ def test_silu_over_its_range(gpu, m):
 
 SHAPES = [(1, 1, 1), (1, 17, 32), (2, 16, 129), (3, 203, 100), (15, 64, 896), (16, 16, 128), (17, 33, 257), (31, 1, 640),
           (33, 130, 1040), (64, 96, 384), (65, 257, 1000), (130, 131, 512), (300, 65, 130), (1, 896, 4864), (5, 1152, 896),
-          (129, 128, 4864), (257, 384, 896)]
+          (129, 128, 4864), (257, 384, 896), (5, 4997, 1600), (16, 5000, 2177), (50, 1370, 1700), (1, 4513, 4100)]
 
 
 # many outputs: ragged in rows, columns and steps of 128 (4 to 9 of them)
@@ -338,7 +338,7 @@ def test_bad_blocks_stay_in_their_rows(gpu, m, n, k, bits):
         assert np.array_equal(float_bits_of(got[i][~bad]), float_bits_of(clean[i][~bad]))
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 50, 200), (20, 51, 896), (130, 260, 640), (1030, 1101, 640)])
+@pytest.mark.parametrize("m,n,k", [(1, 50, 200), (20, 51, 896), (130, 260, 640), (1030, 1101, 640), (7, 4999, 1700)])
 def test_residual_in_place_and_guards(gpu, m, n, k):
     """y over the residual, on an address of a float, and nothing written outside it."""
     from nanocompile_amd import hip, kernels

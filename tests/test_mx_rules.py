@@ -7,8 +7,9 @@ import pytest
 from tests import test_mx_gpu
 from tests.test_rules import run  # noqa: F401 (the fixture)
 
-ROW, LONG_ROW, SPLIT, JOINED, SMALL, DEEP, MEDIUM, MEDIUM_DEEP, LARGE = range(9)
-MISSING = {(4, 1): {MEDIUM}, (8, 1): set(), (4, 2): {MEDIUM, MEDIUM_DEEP}, (8, 2): {MEDIUM_DEEP}}
+ROW, LONG_ROW, WIDE_ROW, SPLIT, JOINED, SMALL, DEEP, MEDIUM, MEDIUM_DEEP, LARGE = range(10)
+MISSING = {(4, 1): {WIDE_ROW, MEDIUM}, (8, 1): set(), (4, 2): {WIDE_ROW, MEDIUM, MEDIUM_DEEP},
+           (8, 2): {WIDE_ROW, MEDIUM_DEEP}}
 
 
 def kinds(run, cases):
@@ -18,7 +19,8 @@ def kinds(run, cases):
 
 
 def test_where_each_measured_quicker(run):  # noqa: F811
-    cases = [(4, 1, 2, 4864, 896, ROW), (4, 1, 3, 726, 6801, LONG_ROW), (8, 1, 13, 4096, 4096, LONG_ROW),
+    cases = [(4, 1, 2, 4864, 896, ROW), (4, 1, 3, 726, 6801, LONG_ROW), (8, 1, 13, 4096, 4096, LONG_ROW), (8, 1, 8, 8192, 8192, WIDE_ROW),
+             (8, 1, 163, 896, 4864, ROW),
              (4, 1, 76, 1152, 896, ROW), (4, 1, 199, 918, 287, SPLIT), (4, 1, 2021, 161, 1104, SPLIT),
              (4, 1, 146, 896, 4864, JOINED), (8, 2, 53, 3195, 5597, JOINED), (4, 2, 190, 3139, 2592, DEEP),
              (4, 1, 2162, 896, 4864, DEEP), (4, 2, 465, 4864, 896, SMALL), (4, 1, 923, 8192, 2048, MEDIUM_DEEP),
@@ -33,14 +35,14 @@ def test_where_each_measured_quicker(run):  # noqa: F811
 def test_the_products_tests_reach_every_kind(run, bits, weights):  # noqa: F811
     shapes = test_mx_gpu.SHAPES + test_mx_gpu.WIDE + test_mx_gpu.LONG + test_mx_gpu.SHORT + test_mx_gpu.TILES
     reached = set(kinds(run, [(bits, weights, *shape) for shape in shapes]))
-    assert reached == set(range(9)) - MISSING[bits, weights]
+    assert reached == set(range(10)) - MISSING[bits, weights]
 
 
 @pytest.mark.parametrize("weights", [1, 2])
 @pytest.mark.parametrize("bits", [4, 8])
 def test_one_shape_of_each_kind(run, bits, weights):  # noqa: F811
     reached = set(kinds(run, [(bits, weights, *shape) for shape in test_mx_gpu.KINDS]))
-    assert reached == set(range(JOINED, 9)) - MISSING[bits, weights]
+    assert reached == set(range(JOINED, 10)) - MISSING[bits, weights]
 
 
 def test_what_the_kernels_need(run):  # noqa: F811
